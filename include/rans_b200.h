@@ -36,7 +36,8 @@ extern "C" {
 typedef struct CUstream_st* cudaStream_t;
 #endif
 
-#define RANS_B200_ABI_VERSION 3   /* 2: escape-code entry points, rans_gemv_step_kernels; 3: chain launcher */
+#define RANS_B200_ABI_VERSION 4   /* 2: escape-code entry points, rans_gemv_step_kernels; 3: chain launcher;
+                                     4: key-value cache (rans_kv.h) */
 
 /* ---------------------------------------------------------------- drop-in
  * The three entry points of the reference library, same names, argument

@@ -1,0 +1,828 @@
+// Attention of one new token per sequence over a paged key-value cache, split
+// over the cache's length and joined.
+//
+// For a kv head and its group of query heads q_0..q_{G-1} the kernel computes,
+// over tiles of 16 tokens and with the running maximum m and sum l of a softmax,
+//
+//     S^T = K Q^T            (tokens x heads)
+//     P^T = exp2(S^T c - m)  (c = scale * log2 e)
+//     O^T = O^T 2^(m_old - m) + V^T P^T   (dim x heads)
+//
+// Both products take the cache as the 16-row operand of mma.m16n8k16 and the
+// heads as its 8 columns, so a group of 8 heads wastes no tensor work and a tile's
+// scores lie in four registers.  The work is bound by reading K and V once (4 G
+// flops a byte at 16 bits, far below the tensor rate even of this instruction).
+//
+// Operands go from global memory straight to registers, 16 bytes a lane: the
+// order of the contraction index is free, so a lane's 8 consecutive values of a
+// key row are its operands of two consecutive k-steps, with
+// Q's registers loaded in the same order; and a lane that reads the same 8
+// columns of four value rows gets V^T's operands by one byte permute each.
+// Nothing is staged, so no warp waits for another while it streams.
+//
+// Work is shared out by tiles: the grid's warps get equal runs of the list of all
+// (sequence, kv head, tile), whatever the lengths are.  A warp that has a whole
+// (sequence, kv head) writes its output; else the block joins its warps' parts in
+// shared memory, and the last block to finish a (sequence, kv head) joins the
+// blocks' parts (always in the order of the tiles, so results do not depend on
+// which block that is).
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_runtime.h>
+
+#include "rans_kv_common.h"
+
+namespace rb200kv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 16;
+// The maximum is only raised when a score passes it by this much (in powers of
+// two): probabilities then stay below 2^8, harmless in bf16, fp16 and fp32.
+constexpr float kSlack = 8.0f;
+
+struct AttendArgs {
+    RansKvCache c;
+    const char* q;
+    int64_t q_batch, q_head;     // bytes
+    void* out;
+    float* log_sum;
+    float scale_log2;
+    int heads, group;            // group = heads / kv_heads
+    int subs, sub_heads;         // a group is cut into `subs` parts of at most sub_heads
+    int q_half;                  // q and out are fp16 (else bf16)
+    int weigh;
+    int* counter;                // [batch * kv_heads * subs]
+    float2* stats;               // [batch * heads]: maximum (log2) and 1 / sum
+    float* part;                 // [grid][2][HP][D + 2]
+    float* scores;               // [tile][16][HP], scaled, log2
+    int64_t score_tiles;
+};
+
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
+template <bool HALF>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    if constexpr (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (HALF) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_as(int half, float lo, float hi) {
+    return half ? pack2<true>(lo, hi) : pack2<false>(lo, hi);
+}
+
+// Two e2m1 codes (one byte) as fp16, exact.
+__device__ __forceinline__ uint32_t e2m1_to_half2(uint32_t byte) {
+    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1);
+    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+// 2^e of a scale byte e + 127 (255: infinity, whose product with the zero codes of such a block is NaN).
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// The factors that turn two tokens' e2m1 codes, read as the low bits of bf16
+// (value * 2^-126), into value * 2^(e - 63): 2^(63 + e), a bf16 for every e the
+// format has.  The remaining 2^63 is applied to the output.
+__device__ __forceinline__ uint32_t factor2(uint32_t byte0, uint32_t byte1) {
+    return (min(byte0 + 63u, 255u) << 7) | (min(byte1 + 63u, 255u) << 23);
+}
+
+template <int KIND, int D, int NT>
+struct Attend {
+    static constexpr bool kFp4 = KIND == RANS_KV_MXFP4;
+    [[maybe_unused]] static constexpr bool kHalfK = KIND != RANS_KV_BF16;      // operands of S (4-bit values are exact in fp16)
+    static constexpr bool kHalfV = KIND == RANS_KV_FP16;      // operands of O (4-bit values times their scale need bf16's range)
+    static constexpr int HP = NT * 8;                         // heads of a tile, padded
+    static constexpr int kChunks = D / 32;                    // 32 values of a row
+    static constexpr int kWarps = (NT == 2 && D == 128) || D == 256 ? 4 : 8;
+    static constexpr int kBlocksPerSm = 2;
+    static constexpr int kRow = D + 4;                        // a head's part in shared memory
+
+    struct Smem {
+        float o[kWarps * 2][HP][kRow];
+        float m[kWarps * 2][HP];
+        float l[kWarps * 2][HP];
+        int tag[kWarps * 2];
+        int last[2];
+        int warp_sum[kWarps];
+        int pre[RANS_KV_MAX_BATCH + 1];
+    };
+
+    // One tile's rows as they come from memory.
+    struct Raw {
+        uint4 k[kFp4 ? 1 : 2][kFp4 ? 1 : kChunks];
+        uint4 v[kFp4 ? 1 : 4][kFp4 ? 1 : D / 64];
+        uint32_t kw[kFp4 ? 2 : 1][kFp4 ? kChunks : 1];        // codes of rows g, g + 8: word n = block n
+        uint32_t vw[kFp4 ? 4 : 1][kFp4 ? D / 64 : 1];
+        uint32_t ks[kFp4 ? 2 : 1][kFp4 ? (D + 127) / 128 : 1];
+        uint32_t vs[kFp4 ? 4 : 1];
+        int valid;                                            // tokens of the tile
+    };
+
+    static __device__ __forceinline__ void load(Raw& r, const AttendArgs& a, int b, int h, int n, int tile, int lane) {
+        const RansKvCache& c = a.c;
+        const int g = lane >> 2, q4 = lane & 3;
+        const int t0 = tile * kTile, in_page = t0 / c.page, slot = t0 - in_page * c.page;
+        const int p = checked_page(c, b, in_page);
+        r.valid = p < 0 ? 0 : min(n - t0, kTile);
+        const int64_t pg = p < 0 ? 0 : p;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const int vrow[4] = {2 * q4, 2 * q4 + 1, 2 * q4 + 8, 2 * q4 + 9};
+        if constexpr (!kFp4) {
+            const char* kp = static_cast<const char*>(c.k) + pg * c.k_page + h * c.k_head + slot * c.k_slot + q4 * 16;
+            const char* vp = static_cast<const char*>(c.v) + pg * c.v_page + h * c.v_head + slot * c.v_slot + g * 16;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j)
+                    r.k[i][j] = g + 8 * i < r.valid ? load16(kp + (g + 8 * i) * c.k_slot + j * 64) : zero;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j)
+                    r.v[i][j] = vrow[i] < r.valid ? load16(vp + vrow[i] * c.v_slot + j * 128) : zero;
+        } else {
+            const int64_t row0 = (pg * c.kv_heads + h) * c.page + slot;
+            const uint8_t* kp = static_cast<const uint8_t*>(c.k) + row0 * (D / 2) + q4 * (D / 8);
+            const uint8_t* vp = static_cast<const uint8_t*>(c.v) + row0 * (D / 2) + g * (D / 16);
+            const uint8_t* ksp = c.k_scale + row0 * kChunks;
+            const uint8_t* vsp = c.v_scale + row0 * kChunks + (g & 1) * (D / 64);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = g + 8 * i;
+                const bool in = t < r.valid;
+#pragma unroll
+                for (int j = 0; j < kChunks; j += 4) {
+                    if constexpr (kChunks >= 4) {
+                        const uint4 w = in ? load16(kp + t * (D / 2) + j * 4) : zero;
+                        r.kw[i][j] = w.x; r.kw[i][j + 1] = w.y; r.kw[i][j + 2] = w.z; r.kw[i][j + 3] = w.w;
+                        r.ks[i][j / 4] = in ? __ldg(reinterpret_cast<const uint32_t*>(ksp + t * kChunks + j)) : 0;
+                    } else {
+                        const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(kp + t * (D / 2))) : make_uint2(0, 0);
+                        r.kw[i][0] = w.x; r.kw[i][1] = w.y;
+                        r.ks[i][0] = in ? __ldg(reinterpret_cast<const uint16_t*>(ksp + t * kChunks)) : 0;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = vrow[i];
+                const bool in = t < r.valid;
+                if constexpr (D == 256) {
+                    const uint4 w = in ? load16(vp + t * (D / 2)) : zero;
+                    r.vw[i][0] = w.x; r.vw[i][1] = w.y; r.vw[i][2] = w.z; r.vw[i][3] = w.w;
+                    r.vs[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(vsp + t * kChunks)) : 0;
+                } else if constexpr (D == 128) {
+                    const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(vp + t * (D / 2))) : make_uint2(0, 0);
+                    r.vw[i][0] = w.x; r.vw[i][1] = w.y;
+                    r.vs[i] = in ? __ldg(reinterpret_cast<const uint16_t*>(vsp + t * kChunks)) : 0;
+                } else {
+                    r.vw[i][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(vp + t * (D / 2))) : 0;
+                    r.vs[i] = in ? __ldg(vsp + t * kChunks) : 0;
+                }
+            }
+        }
+    }
+
+    struct State {
+        float o[D / 16][NT][4];
+        float m[NT][2], l[NT][2];
+        uint4 q[NT][kChunks];
+        float qs[kFp4 ? NT : 1][2];      // 4-bit: the powers of two taken out of the two heads' queries, times scale
+    };
+
+    // The queries of a head group, in the order of load()'s key values.  For 4-bit
+    // keys they become fp16: each head's largest value is first brought to
+    // [2^14, 2^15) by a power of two, so that nothing overflows and what is lost is
+    // below 2^-38 of it.
+    static __device__ __forceinline__ void begin(State& s, const AttendArgs& a, int b, int head0, int heads, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const bool in = t * 8 + g < heads;
+            const char* qp = a.q + b * a.q_batch + (int64_t)(head0 + t * 8 + g) * a.q_head + q4 * 16;
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) s.q[t][j] = in ? load16(qp + j * 64) : make_uint4(0, 0, 0, 0);
+            if constexpr (kFp4) {
+                auto unpack = [&](uint32_t w) {
+                    return a.q_half ? __half22float2(*reinterpret_cast<__half2*>(&w))
+                                    : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+                };
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const float2 f = unpack((&s.q[t][j].x)[w]);
+                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                const int e = top > 0.0f && top <= 3.4e38f ? min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 113) : 0;
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const float2 f = unpack((&s.q[t][j].x)[w]);
+                        (&s.q[t][j].x)[w] = pack2<true>(f.x * down, f.y * down);
+                    }
+                // a lane's scores are of heads 2 q4 and 2 q4 + 1
+                s.qs[t][0] = __shfl_sync(~0u, up, (2 * q4) * 4) * a.scale_log2;
+                s.qs[t][1] = __shfl_sync(~0u, up, (2 * q4 + 1) * 4) * a.scale_log2;
+            }
+            s.m[t][0] = s.m[t][1] = -INFINITY;
+            s.l[t][0] = s.l[t][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) s.o[i][t][0] = s.o[i][t][1] = s.o[i][t][2] = s.o[i][t][3] = 0.0f;
+        }
+    }
+
+    static __device__ __forceinline__ void step(State& s, const Raw& r, const AttendArgs& a, int64_t x, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
+        float sc[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
+        if constexpr (!kFp4) {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                const uint4 k0 = r.k[0][j], k1 = r.k[1][j];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    mma<kHalfK>(sc[t], k0.x, k1.x, k0.y, k1.y, s.q[t][j].x, s.q[t][j].y);
+                    mma<kHalfK>(sc[t], k0.z, k1.z, k0.w, k1.w, s.q[t][j].z, s.q[t][j].w);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[t][i] *= a.scale_log2;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                uint32_t w0[4], w1[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w0[i] = e2m1_to_half2((r.kw[0][j] >> (8 * i)) & 255);
+                    w1[i] = e2m1_to_half2((r.kw[1][j] >> (8 * i)) & 255);
+                }
+                const float f0 = scale_of((r.ks[0][j / 4] >> (8 * (j % 4))) & 255);
+                const float f1 = scale_of((r.ks[1][j / 4] >> (8 * (j % 4))) & 255);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma<true>(d, w0[0], w1[0], w0[1], w1[1], s.q[t][j].x, s.q[t][j].y);
+                    mma<true>(d, w0[2], w1[2], w0[3], w1[3], s.q[t][j].z, s.q[t][j].w);
+                    sc[t][0] = fmaf(d[0], f0, sc[t][0]);
+                    sc[t][1] = fmaf(d[1], f0, sc[t][1]);
+                    sc[t][2] = fmaf(d[2], f1, sc[t][2]);
+                    sc[t][3] = fmaf(d[3], f1, sc[t][3]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                sc[t][0] *= s.qs[t][0]; sc[t][1] *= s.qs[t][1];
+                sc[t][2] *= s.qs[t][0]; sc[t][3] *= s.qs[t][1];
+            }
+        }
+        bool raise_max = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (g >= r.valid) sc[t][0] = sc[t][1] = -INFINITY;
+            if (g + 8 >= r.valid) sc[t][2] = sc[t][3] = -INFINITY;
+            if (a.weigh && x < a.score_tiles) {
+                float* p = a.scores + (x * kTile + g) * HP + t * 8 + 2 * q4;
+                *reinterpret_cast<float2*>(p) = make_float2(sc[t][0], sc[t][1]);
+                *reinterpret_cast<float2*>(p + 8 * HP) = make_float2(sc[t][2], sc[t][3]);
+            }
+            raise_max |= fmaxf(sc[t][0], sc[t][2]) > s.m[t][0] + kSlack || fmaxf(sc[t][1], sc[t][3]) > s.m[t][1] + kSlack;
+        }
+        if (__any_sync(~0u, raise_max)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(sc[t][e], sc[t][e + 2]);
+                    m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+                    m = fmaxf(m, s.m[t][e]);
+                    const float f = m == -INFINITY ? 1.0f : exp2_fast(s.m[t][e] - m);
+                    s.m[t][e] = m;
+                    s.l[t][e] *= f;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        s.o[i][t][e] *= f;
+                        s.o[i][t][e + 2] *= f;
+                    }
+                }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float m0 = s.m[t][0] == -INFINITY ? 0.0f : s.m[t][0], m1 = s.m[t][1] == -INFINITY ? 0.0f : s.m[t][1];
+            const float p0 = exp2_fast(sc[t][0] - m0), p1 = exp2_fast(sc[t][1] - m1);
+            const float p2 = exp2_fast(sc[t][2] - m0), p3 = exp2_fast(sc[t][3] - m1);
+            s.l[t][0] += p0 + p2;
+            s.l[t][1] += p1 + p3;
+            pb[t][0] = transpose8x8(pack2<kHalfV>(p0, p1));
+            pb[t][1] = transpose8x8(pack2<kHalfV>(p2, p3));
+        }
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            if constexpr (!kFp4) {
+                const uint32_t* v0 = &r.v[0][j].x;
+                const uint32_t* v1 = &r.v[1][j].x;
+                const uint32_t* v2 = &r.v[2][j].x;
+                const uint32_t* v3 = &r.v[3][j].x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
+                    const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) mma<kHalfV>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                }
+            } else {
+                const uint32_t lo01 = __byte_perm(r.vw[0][j], r.vw[1][j], 0x5410), hi01 = __byte_perm(r.vw[0][j], r.vw[1][j], 0x7632);
+                const uint32_t lo23 = __byte_perm(r.vw[2][j], r.vw[3][j], 0x5410), hi23 = __byte_perm(r.vw[2][j], r.vw[3][j], 0x7632);
+                const uint32_t f01 = factor2((r.vs[0] >> (8 * j)) & 255, (r.vs[1] >> (8 * j)) & 255);
+                const uint32_t f23 = factor2((r.vs[2] >> (8 * j)) & 255, (r.vs[3] >> (8 * j)) & 255);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    auto value = [&](uint32_t w, uint32_t f) {
+                        const uint32_t y = w << (12 - 4 * i);         // the code in the top bits of each half
+                        const uint32_t bits = (y & 0x80008000u) | ((y >> 6) & 0x01C001C0u);
+                        const __nv_bfloat162 z = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), *reinterpret_cast<const __nv_bfloat162*>(&f));
+                        return *reinterpret_cast<const uint32_t*>(&z);
+                    };
+                    const uint32_t a0 = value(lo01, f01), a1 = value(hi01, f01), a2 = value(lo23, f23), a3 = value(hi23, f23);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) mma<kHalfV>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                }
+            }
+        }
+    }
+
+    // First of the 8 consecutive values that o[j * 4 .. j * 4 + 3] of lane group g hold, and which
+    // accumulator holds value e: 16-bit rows pair neighbours, 4-bit rows pair e and e + 4.
+    static __device__ __forceinline__ int first_d(int j, int g) {
+        if constexpr (!kFp4) return j * 64 + g * 8;
+        const int w = g * (D / 64) + j;
+        return (w % kChunks) * 32 + (w / kChunks) * 8;
+    }
+    static __device__ __forceinline__ float value_of(const State& s, int j, int t, int head, int e) {
+        return kFp4 ? s.o[j * 4 + (e & 3)][t][head + 2 * (e >> 2)] : s.o[j * 4 + (e >> 1)][t][head + 2 * (e & 1)];
+    }
+    // What the output still has to be multiplied by.
+    static __device__ __forceinline__ float out_scale() { return kFp4 ? 9.223372036854775808e18f : 1.0f; }
+
+    static __device__ __forceinline__ void finish_head(const AttendArgs& a, int b, int head, float m, float l) {
+        const int64_t i = (int64_t)b * a.heads + head;
+        if (a.log_sum != nullptr) a.log_sum[i] = l > 0.0f || l != l ? m * 0.6931471805599453f + logf(l) : -INFINITY;
+        if (a.weigh) a.stats[i] = make_float2(m == -INFINITY ? 0.0f : m, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+    }
+
+    // A warp's state: into `part` (smem) or, when it is the whole of a (sequence, head group), to the output.
+    static __device__ __forceinline__ void reduce_sum(State& s) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s.l[t][e] += __shfl_xor_sync(~0u, s.l[t][e], 4);
+                s.l[t][e] += __shfl_xor_sync(~0u, s.l[t][e], 8);
+                s.l[t][e] += __shfl_xor_sync(~0u, s.l[t][e], 16);
+            }
+    }
+
+    static __device__ __forceinline__ void write_out(const State& s, const AttendArgs& a, int b, int head0, int heads, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int head = t * 8 + 2 * q4 + e;
+                if (head >= heads) continue;
+                const float l = s.l[t][e], f = l > 0.0f || l != l ? out_scale() / l : 0.0f;
+                char* o = static_cast<char*>(a.out) + ((int64_t)b * a.heads + head0 + head) * D * 2;
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) {
+                    uint4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        (&w.x)[i] = pack_as(a.q_half, value_of(s, j, t, e, 2 * i) * f, value_of(s, j, t, e, 2 * i + 1) * f);
+                    *reinterpret_cast<uint4*>(o + first_d(j, g) * 2) = w;
+                }
+                if (g == 0) finish_head(a, b, head0 + head, s.m[t][e], l);
+            }
+    }
+
+    static __device__ __forceinline__ void write_part(const State& s, Smem& sm, int slot, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int head = t * 8 + 2 * q4 + e;
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<float4*>(&sm.o[slot][head][first_d(j, g) + 4 * i]) =
+                            make_float4(value_of(s, j, t, e, 4 * i), value_of(s, j, t, e, 4 * i + 1),
+                                        value_of(s, j, t, e, 4 * i + 2), value_of(s, j, t, e, 4 * i + 3));
+                if (g == 0) {
+                    sm.m[slot][head] = s.m[t][e];
+                    sm.l[slot][head] = s.l[t][e];
+                }
+            }
+    }
+
+    static __device__ __forceinline__ void store_joined(const AttendArgs& a, int b, int head, int d, float4 o, float m, float l) {
+        const float f = l > 0.0f || l != l ? out_scale() / l : 0.0f;
+        uint2 w;
+        w.x = pack_as(a.q_half, o.x * f, o.y * f);
+        w.y = pack_as(a.q_half, o.z * f, o.w * f);
+        *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + (((int64_t)b * a.heads + head) * D + d) * 2) = w;
+        if (d == 0) finish_head(a, b, head, m, l);
+    }
+};
+
+__device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
+template <int KIND, int D, int NT>
+__global__ void __launch_bounds__(Attend<KIND, D, NT>::kWarps * 32, Attend<KIND, D, NT>::kBlocksPerSm)
+attend_kernel(const __grid_constant__ AttendArgs a) {
+    using A = Attend<KIND, D, NT>;
+    constexpr int HP = A::HP, W = A::kWarps, kThreads = W * 32;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    typename A::Smem& sm = *reinterpret_cast<typename A::Smem*>(smem_raw);
+    const RansKvCache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int segs = c.kv_heads * a.subs;               // (kv head, part of its group) of one sequence
+
+    // Tiles in front of each sequence.
+    {
+        const int per = (c.batch + kThreads - 1) / kThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
+        int sum = 0;
+        for (int b = b0; b < b1; ++b) sum += (checked_length(c, b) + kTile - 1) / kTile * segs;
+        int inc = sum;
+#pragma unroll
+        for (int i = 1; i < 32; i *= 2) {
+            const int y = __shfl_up_sync(~0u, inc, i);
+            if (lane >= i) inc += y;
+        }
+        if (lane == 31) sm.warp_sum[warp] = inc;
+        if (lane < 2) sm.tag[warp * 2 + lane] = -1;
+        __syncthreads();
+        int at = inc - sum;
+        for (int w = 0; w < warp; ++w) at += sm.warp_sum[w];
+        for (int b = b0; b < b1; ++b) {
+            sm.pre[b] = at;
+            at += (checked_length(c, b) + kTile - 1) / kTile * segs;
+        }
+        if (b1 == c.batch && b0 < b1) sm.pre[c.batch] = at;
+        __syncthreads();
+    }
+    const int total = sm.pre[c.batch];
+    auto tiles_of = [&](int b) { return (sm.pre[b + 1] - sm.pre[b]) / segs; };
+
+    // Sequences without tokens.
+    for (int b = blockIdx.x; b < c.batch; b += gridDim.x)
+        if (sm.pre[b + 1] == sm.pre[b])
+            for (int i = tid; i < a.heads * (D / 8); i += kThreads) {
+                reinterpret_cast<uint4*>(a.out)[(int64_t)b * a.heads * (D / 8) + i] = make_uint4(0, 0, 0, 0);
+                if (i < a.heads && a.log_sum != nullptr) a.log_sum[(int64_t)b * a.heads + i] = -INFINITY;
+            }
+
+    const int blocks = min((int)gridDim.x, (total + W - 1) / W);       // each of their warps has a tile
+    if ((int)blockIdx.x >= blocks) return;
+    const int x0 = (int)((int64_t)total * blockIdx.x / blocks), x1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
+    int x = x0 + (int)((int64_t)(x1 - x0) * warp / W);
+    const int xe = x0 + (int)((int64_t)(x1 - x0) * (warp + 1) / W);
+
+    if (x < xe) {
+        int lo = 0, hi = c.batch;                       // the sequence of tile x: pre[lo] <= x < pre[lo + 1]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (sm.pre[mid] <= x) lo = mid; else hi = mid;
+        }
+        int b = lo, nt = tiles_of(b), seg = (x - sm.pre[b]) / nt, tile = (x - sm.pre[b]) - seg * nt, parts = 0;
+        typename A::State s;
+        while (x < xe) {
+            const int end = min(tile + (xe - x), nt);
+            const int h = seg / a.subs, sub = seg - h * a.subs;
+            const int head0 = h * a.group + sub * a.sub_heads, heads = min(a.sub_heads, a.group - sub * a.sub_heads);
+            const int n = checked_length(c, b);
+            const bool whole = tile == 0 && end == nt;
+            A::begin(s, a, b, head0, heads, lane);
+            for (; tile < end; ++tile, ++x) {
+                typename A::Raw r;
+                A::load(r, a, b, h, n, tile, lane);
+                A::step(s, r, a, x, lane);
+            }
+            A::reduce_sum(s);
+            if (whole) {
+                A::write_out(s, a, b, head0, heads, lane);
+            } else {
+                A::write_part(s, sm, warp * 2 + parts, lane);
+                if (lane == 0) sm.tag[warp * 2 + parts] = b * segs + seg;
+                ++parts;
+            }
+            tile = 0;
+            if (++seg == segs) {
+                seg = 0;
+                do ++b; while (b < c.batch && sm.pre[b + 1] == sm.pre[b]);
+                if (b < c.batch) nt = tiles_of(b);
+            }
+        }
+    }
+    __syncthreads();
+
+    // Join the warps' parts of each (sequence, head group); what this block has not all of goes to `part`.
+    constexpr int kVec = HP * (D / 4);
+    int open[2] = {-1, -1};
+    for (int i0 = 0; i0 < W * 2;) {
+        const int tag = sm.tag[i0];
+        if (tag < 0) { ++i0; continue; }
+        int i1 = i0 + 1;
+        while (i1 < W * 2 && (sm.tag[i1] == tag || sm.tag[i1] < 0)) ++i1;
+        const int b = tag / segs, seg = tag - b * segs, nt = tiles_of(b), start = sm.pre[b] + seg * nt;
+        const int h = seg / a.subs, sub = seg - h * a.subs;
+        const int head0 = h * a.group + sub * a.sub_heads, heads = min(a.sub_heads, a.group - sub * a.sub_heads);
+        const bool whole = start >= x0 && start + nt <= x1;
+        const int slot = start <= x0 ? 0 : 1;
+        if (!whole) open[slot] = tag;
+        float* part = a.part + (int64_t)(blockIdx.x * 2 + slot) * HP * (D + 2);
+        for (int v = tid; v < kVec; v += kThreads) {
+            const int head = v / (D / 4), d = v % (D / 4) * 4;
+            if (head >= heads) break;
+            float top = -INFINITY;
+            for (int i = i0; i < i1; ++i)
+                if (sm.tag[i] >= 0) top = fmaxf(top, sm.m[i][head]);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float l = 0.0f;
+            for (int i = i0; i < i1; ++i) {
+                if (sm.tag[i] < 0) continue;
+                const float f = join_factor(sm.m[i][head], top);
+                const float4 y = *reinterpret_cast<const float4*>(&sm.o[i][head][d]);
+                o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+                l = fmaf(sm.l[i][head], f, l);
+            }
+            if (whole) {
+                A::store_joined(a, b, head0 + head, d, o, top, l);
+            } else {
+                __stcg(reinterpret_cast<float4*>(part + head * D + d), o);
+                if (d == 0) {
+                    __stcg(part + HP * D + head * 2, top);
+                    __stcg(part + HP * D + head * 2 + 1, l);
+                }
+            }
+        }
+        i0 = i1;
+    }
+
+    // The last block of a (sequence, head group) joins the blocks' parts.
+    __threadfence();
+    __syncthreads();
+    auto block_of = [&](int tile) { return (int)((((int64_t)tile + 1) * blocks - 1) / total); };
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            sm.last[i] = 0;
+            if (open[i] < 0) continue;
+            const int b = open[i] / segs, seg = open[i] - b * segs, nt = tiles_of(b), start = sm.pre[b] + seg * nt;
+            const int splits = block_of(start + nt - 1) - block_of(start) + 1;
+            if (atomicAdd(a.counter + open[i], 1) == splits - 1) {
+                a.counter[open[i]] = 0;
+                sm.last[i] = 1;
+            }
+        }
+        __threadfence();
+    }
+    __syncthreads();
+    for (int i = 0; i < 2; ++i) {
+        if (!sm.last[i]) continue;
+        const int b = open[i] / segs, seg = open[i] - b * segs, nt = tiles_of(b), start = sm.pre[b] + seg * nt;
+        const int h = seg / a.subs, sub = seg - h * a.subs;
+        const int head0 = h * a.group + sub * a.sub_heads, heads = min(a.sub_heads, a.group - sub * a.sub_heads);
+        const int c0 = block_of(start), c1 = block_of(start + nt - 1);
+        const int slot0 = (int64_t)total * c0 / blocks >= start ? 0 : 1;     // only the first block's part may be its second
+        auto part_of = [&](int k) { return a.part + (int64_t)(k * 2 + (k == c0 ? slot0 : 0)) * HP * (D + 2); };
+        for (int v = tid; v < kVec; v += kThreads) {
+            const int head = v / (D / 4), d = v % (D / 4) * 4;
+            if (head >= heads) break;
+            float top = -INFINITY;
+            for (int k = c0; k <= c1; ++k) top = fmaxf(top, __ldcg(part_of(k) + HP * D + head * 2));
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float l = 0.0f;
+#pragma unroll 4
+            for (int k = c0; k <= c1; ++k) {
+                const float* p = part_of(k);
+                const float f = join_factor(__ldcg(p + HP * D + head * 2), top);
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(p + head * D + d));
+                o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+                l = fmaf(__ldcg(p + HP * D + head * 2 + 1), f, l);
+            }
+            A::store_joined(a, b, head0 + head, d, o, top, l);
+        }
+    }
+}
+
+// weight[t] += sum over the query heads of exp2(score - m) / l, one thread per token and kv head.
+constexpr int kWeighThreads = 256;
+
+__global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_constant__ AttendArgs a, int hp) {
+    __shared__ int pre[RANS_KV_MAX_BATCH + 1];
+    __shared__ int warp_sum[kWeighThreads / 32];
+    const RansKvCache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (c.batch + kWeighThreads - 1) / kWeighThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) sum += (checked_length(c, b) + kTile - 1) / kTile;
+    int inc = sum;
+#pragma unroll
+    for (int i = 1; i < 32; i *= 2) {
+        const int y = __shfl_up_sync(~0u, inc, i);
+        if (lane >= i) inc += y;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < warp; ++w) at += warp_sum[w];
+    for (int b = b0; b < b1; ++b) {
+        pre[b] = at;
+        at += (checked_length(c, b) + kTile - 1) / kTile;
+    }
+    if (b1 == c.batch && b0 < b1) pre[c.batch] = at;
+    __syncthreads();
+    const int total = pre[c.batch];                     // tiles of one head of every sequence
+    const int64_t all = (int64_t)total * c.kv_heads * kTile;
+    for (int64_t i = (int64_t)blockIdx.x * kWeighThreads + tid; i < all; i += (int64_t)gridDim.x * kWeighThreads) {
+        const int64_t xt = i / kTile;                   // (sequence, kv head, tile)
+        int lo = 0, hi = c.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if ((int64_t)pre[mid] * c.kv_heads <= xt) lo = mid; else hi = mid;
+        }
+        const int b = lo, nt = pre[b + 1] - pre[b];
+        const int64_t in = xt - (int64_t)pre[b] * c.kv_heads;
+        const int h = (int)(in / nt), tile = (int)(in - (int64_t)h * nt), t = tile * kTile + (int)(i % kTile);
+        if (t >= checked_length(c, b)) continue;
+        const int p = checked_page(c, b, t / c.page);
+        if (p < 0) continue;
+        float add = 0.0f;
+        for (int sub = 0; sub < a.subs; ++sub) {
+            const int64_t x = (int64_t)pre[b] * c.kv_heads * a.subs + ((int64_t)h * a.subs + sub) * nt + tile;
+            if (x >= a.score_tiles) { raise(c, RANS_KV_BAD_LENGTH); break; }
+            const float* s = a.scores + (x * kTile + i % kTile) * hp;
+            const int first = sub * a.sub_heads, heads = min(a.sub_heads, a.group - first);
+            const float2* st = a.stats + (int64_t)b * a.heads + h * a.group + first;
+            for (int k = 0; k < heads; ++k) add = fmaf(exp2_fast(s[k] - st[k].x), st[k].y, add);
+        }
+        float* w = c.weight + ((int64_t)p * c.kv_heads + h) * c.page + t % c.page;
+        *w += add;
+    }
+}
+
+struct Plan {
+    int nt, subs, sub_heads;
+    int64_t counter, stats, part, scores, bytes, score_tiles;
+};
+
+constexpr int kGrid = kSms * 2;
+
+bool make_plan(const RansKvCache& c, int heads, int weigh, Plan& p) {
+    if (heads < 1 || heads % c.kv_heads != 0) return false;
+    const int group = heads / c.kv_heads, most = c.dim == 256 ? 8 : 16;
+    p.subs = (group + most - 1) / most;
+    if (p.subs > kMaxSubgroups) return false;
+    p.sub_heads = (group + p.subs - 1) / p.subs;
+    p.nt = p.sub_heads > 8 ? 2 : 1;
+    auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+    p.counter = 256;
+    p.stats = counter_bytes(c);
+    p.part = p.stats + up((int64_t)c.batch * heads * 8);
+    p.scores = p.part + up((int64_t)kGrid * 2 * p.nt * 8 * (c.dim + 2) * 4);
+    // every token of every page, and a started tile for each sequence
+    p.score_tiles = weigh ? ((int64_t)c.pages * c.page / kTile + c.batch) * c.kv_heads * p.subs : 0;
+    p.bytes = p.scores + up(p.score_tiles * kTile * p.nt * 8 * 4);
+    return true;
+}
+
+template <int KIND, int D, int NT>
+int launch(const AttendArgs& a, cudaStream_t stream) {
+    using A = Attend<KIND, D, NT>;
+    auto kernel = attend_kernel<KIND, D, NT>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename A::Smem));
+    if (e != cudaSuccess) return (int)e;
+    kernel<<<kGrid, A::kWarps * 32, sizeof(typename A::Smem), stream>>>(a);
+    return (int)cudaGetLastError();
+}
+
+template <int KIND>
+int launch_kind(const AttendArgs& a, int nt, cudaStream_t stream) {
+    switch (a.c.dim) {
+        case 64: return nt == 1 ? launch<KIND, 64, 1>(a, stream) : launch<KIND, 64, 2>(a, stream);
+        case 128: return nt == 1 ? launch<KIND, 128, 1>(a, stream) : launch<KIND, 128, 2>(a, stream);
+        case 256: return launch<KIND, 256, 1>(a, stream);
+        default: return -1;
+    }
+}
+
+}  // namespace
+}  // namespace rb200kv
+
+using namespace rb200kv;
+
+extern "C" int64_t rans_kv_counter_bytes(const RansKvCache* c) {
+    if (c == nullptr || c->batch < 1 || c->batch > RANS_KV_MAX_BATCH || c->kv_heads < 1) return -2;
+    return counter_bytes(*c);
+}
+
+extern "C" int64_t rans_kv_attend_bytes(const RansKvCache* c, int heads, int weigh) {
+    if (rans_kv_counter_bytes(c) < 0 || c->pages < 1 || c->page < 16) return -2;
+    Plan p;
+    return make_plan(*c, heads, weigh, p) ? p.bytes : -2;
+}
+
+extern "C" int rans_kv_attend(const RansKvCache* cache, const void* q, int q_kind, int64_t q_batch, int64_t q_head, int heads,
+                              float scale, void* out, float* log_sum, int weigh, cudaStream_t stream) {
+    const int rc = check_cache(cache);
+    if (rc != 0) return rc;
+    if (q_kind != RANS_KV_BF16 && q_kind != RANS_KV_FP16) return -1;
+    if (cache->kind != RANS_KV_MXFP4 && q_kind != cache->kind) return -1;
+    Plan p;
+    if (!make_plan(*cache, heads, weigh, p)) return -2;
+    if (q == nullptr || out == nullptr || !aligned16(q) || !aligned16(out) || ((q_batch | q_head) & 15)) return -2;
+    if (weigh && cache->weight == nullptr) return -2;
+    if (cache->workspace_bytes < p.bytes) return -3;
+    AttendArgs a{};
+    a.c = *cache;
+    fill_strides(a.c);
+    char* ws = static_cast<char*>(cache->workspace);
+    a.q = static_cast<const char*>(q);
+    a.q_batch = q_batch;
+    a.q_head = q_head;
+    a.out = out;
+    a.log_sum = log_sum;
+    a.scale_log2 = scale * kLog2e;
+    a.heads = heads;
+    a.group = heads / cache->kv_heads;
+    a.subs = p.subs;
+    a.sub_heads = p.sub_heads;
+    a.q_half = q_kind == RANS_KV_FP16;
+    a.weigh = weigh != 0;
+    a.counter = reinterpret_cast<int*>(ws + p.counter);
+    a.stats = reinterpret_cast<float2*>(ws + p.stats);
+    a.part = reinterpret_cast<float*>(ws + p.part);
+    a.scores = reinterpret_cast<float*>(ws + p.scores);
+    a.score_tiles = p.score_tiles;
+    int e;
+    switch (cache->kind) {
+        case RANS_KV_BF16: e = launch_kind<RANS_KV_BF16>(a, p.nt, stream); break;
+        case RANS_KV_FP16: e = launch_kind<RANS_KV_FP16>(a, p.nt, stream); break;
+        default: e = launch_kind<RANS_KV_MXFP4>(a, p.nt, stream); break;
+    }
+    if (e != 0 || !weigh) return e;
+    weigh_kernel<<<kSms * 8, kWeighThreads, 0, stream>>>(a, p.nt * 8);
+    return (int)cudaGetLastError();
+}

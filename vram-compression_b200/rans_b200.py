@@ -31,7 +31,7 @@ M = 1 << SCALE_BITS
 RANS_L = 1 << 16
 OFFSET = 128
 PAD_WORDS = 8
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 _vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 
@@ -92,6 +92,21 @@ def _bind(lib):
     lib.rans_gemv_chain_launch.restype = _i32
     lib.rans_gemv_chain_status.argtypes = [_vp, _vp, _vp]
     lib.rans_gemv_chain_status.restype = _i32
+    # the key-value cache (include/rans_kv.h)
+    lib.rans_kv_counter_bytes.argtypes = [_vp]
+    lib.rans_kv_counter_bytes.restype = _i64
+    lib.rans_kv_attend_bytes.argtypes = [_vp, _i32, _i32]
+    lib.rans_kv_attend_bytes.restype = _i64
+    lib.rans_kv_evict_bytes.argtypes = [_vp, _i32]
+    lib.rans_kv_evict_bytes.restype = _i64
+    lib.rans_kv_append.argtypes = [_vp, _vp, _vp, _i32] + [_i64] * 4 + [_vp, _i32, _vp]
+    lib.rans_kv_append.restype = _i32
+    lib.rans_kv_read.argtypes = [_vp] * 4 + [_i32, _vp]
+    lib.rans_kv_read.restype = _i32
+    lib.rans_kv_attend.argtypes = [_vp, _vp, _i32, _i64, _i64, _i32, ctypes.c_float, _vp, _vp, _i32, _vp]
+    lib.rans_kv_attend.restype = _i32
+    lib.rans_kv_evict.argtypes = [_vp, _i32, _i32, _vp]
+    lib.rans_kv_evict.restype = _i32
     lib.rans_b200_abi_version.argtypes = []
     lib.rans_b200_abi_version.restype = _i32
     return lib
