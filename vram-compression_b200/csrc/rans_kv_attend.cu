@@ -42,6 +42,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 16;
+constexpr int kGrid = kSms;
 // The maximum is only raised when a score passes it by this much (in powers of
 // two): probabilities then stay below 2^8, harmless in bf16, fp16 and fp32.
 constexpr float kSlack = 8.0f;
@@ -59,7 +60,7 @@ struct AttendArgs {
     int weigh;
     int* counter;                // [batch * kv_heads * subs]
     float2* stats;               // [batch * heads]: maximum (log2) and 1 / sum
-    float* part;                 // [grid][2][HP][D + 2]
+    float* part;                 // [grid][2] Attend::Part
     float* scores;               // [tile][16][HP], scaled, log2
     int64_t score_tiles;
 };
@@ -127,123 +128,189 @@ __device__ __forceinline__ uint32_t factor2(uint32_t byte0, uint32_t byte1) {
     return (min(byte0 + 63u, 255u) << 7) | (min(byte1 + 63u, 255u) << 23);
 }
 
+__device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
 template <int KIND, int D, int NT>
 struct Attend {
     static constexpr bool kFp4 = KIND == RANS_KV_MXFP4;
-    [[maybe_unused]] static constexpr bool kHalfK = KIND != RANS_KV_BF16;      // operands of S (4-bit values are exact in fp16)
-    static constexpr bool kHalfV = KIND == RANS_KV_FP16;      // operands of O (4-bit values times their scale need bf16's range)
+    // Operand types: 4-bit keys are exact in fp16 (their scale is applied to the sums); 4-bit values times their scale need bf16's range.
+    static constexpr bool kHalfV = KIND == RANS_KV_FP16;
     static constexpr int HP = NT * 8;                         // heads of a tile, padded
     static constexpr int kChunks = D / 32;                    // 32 values of a row
-    static constexpr int kWarps = (NT == 2 && D == 128) || D == 256 ? 4 : 8;
-    static constexpr int kBlocksPerSm = 2;
+    // One block of an SM's whole register file: fewer parts to join than from several blocks.
+    static constexpr int kWarps = (NT == 2 && D == 128) || D == 256 ? 8 : D == 128 && !kFp4 ? 12 : 16;
     static constexpr int kRow = D + 4;                        // a head's part in shared memory
 
+    // What is left of a run of tiles of one group: O, and the running maximum and sum of each head; a warp's in shared
+    // memory, a block's in the workspace.
+    struct Part {
+        float o[HP][kRow];
+        float2 ml[HP];
+    };
+
     struct Smem {
-        float o[kWarps * 2][HP][kRow];
-        float m[kWarps * 2][HP];
-        float l[kWarps * 2][HP];
-        int tag[kWarps * 2];
-        int last[2];
+        Part part[kWarps * 2];               // the warps' parts: first parts, then second ones
+        int tag[kWarps * 2];                 // the group of each part
+        int first_block[2], last_block[2], last[2];      // of the block's first and last group, if it has only some of it
         int warp_sum[kWarps];
-        int pre[RANS_KV_MAX_BATCH + 1];
+        int pre[RANS_KV_MAX_BATCH + 1];      // tiles of one head in front of each sequence
     };
 
     // One tile's rows as they come from memory.
-    struct Raw {
-        uint4 k[kFp4 ? 1 : 2][kFp4 ? 1 : kChunks];
-        uint4 v[kFp4 ? 1 : 4][kFp4 ? 1 : D / 64];
-        uint32_t kw[kFp4 ? 2 : 1][kFp4 ? kChunks : 1];        // codes of rows g, g + 8: word n = block n
-        uint32_t vw[kFp4 ? 4 : 1][kFp4 ? D / 64 : 1];
-        uint32_t ks[kFp4 ? 2 : 1][kFp4 ? (D + 127) / 128 : 1];
-        uint32_t vs[kFp4 ? 4 : 1];
-        int valid;                                            // tokens of the tile
+    struct RawK {
+        uint4 k[kFp4 ? 1 : 2][kFp4 ? 1 : kChunks];            // rows g, g + 8
+        uint32_t w[kFp4 ? 2 : 1][kFp4 ? kChunks : 1];         // codes: word n = block n
+        uint32_t s[kFp4 ? 2 : 1][kFp4 ? (D + 127) / 128 : 1]; // scale bytes
+    };
+    struct RawV {
+        uint4 v[kFp4 ? 1 : 4][kFp4 ? 1 : D / 64];             // rows 2 q, 2 q + 1, 2 q + 8, 2 q + 9
+        uint32_t w[kFp4 ? 4 : 1][kFp4 ? D / 64 : 1];
+        uint32_t s[kFp4 ? 4 : 1];
     };
 
-    static __device__ __forceinline__ void load(Raw& r, const AttendArgs& a, int b, int h, int n, int tile, int lane) {
-        const RansKvCache& c = a.c;
-        const int g = lane >> 2, q4 = lane & 3;
-        const int t0 = tile * kTile, in_page = t0 / c.page, slot = t0 - in_page * c.page;
-        const int p = checked_page(c, b, in_page);
-        r.valid = p < 0 ? 0 : min(n - t0, kTile);
-        const int64_t pg = p < 0 ? 0 : p;
+    // A lane's place in the tiles of one (sequence, kv head): pointers to its first key and value row of the current
+    // tile.  Within a page they step by 16 rows; the number of the following page is fetched a page ahead.
+    struct Cursor {
+        const char *k, *v, *ks, *vs;
+        int slot, ahead, next, left, valid;      // left: tokens from the tile's first one on; valid: of them in the tile
+
+        __device__ __forceinline__ void at_page(const RansKvCache& c, int h, int p, int lane) {
+            const int g = lane >> 2, q4 = lane & 3;
+            const bool ok = p >= 0 && p < c.pages;
+            if (!ok) raise(c, RANS_KV_BAD_PAGE);
+            valid = ok ? min(left, kTile) : 0;
+            const int64_t pg = ok ? p : 0;
+            if constexpr (!kFp4) {
+                k = static_cast<const char*>(c.k) + pg * c.k_page + h * c.k_head + (slot + g) * c.k_slot + q4 * 16;
+                v = static_cast<const char*>(c.v) + pg * c.v_page + h * c.v_head + (slot + 2 * q4) * c.v_slot + g * 16;
+            } else {
+                const int64_t row = (pg * c.kv_heads + h) * c.page + slot;
+                k = static_cast<const char*>(c.k) + (row + g) * (D / 2) + q4 * (D / 8);
+                v = static_cast<const char*>(c.v) + (row + 2 * q4) * (D / 2) + g * (D / 16);
+                ks = reinterpret_cast<const char*>(c.k_scale) + (row + g) * kChunks;
+                vs = reinterpret_cast<const char*>(c.v_scale) + (row + 2 * q4) * kChunks + (g & 1) * (D / 64);
+            }
+        }
+        __device__ __forceinline__ void fetch_next(const RansKvCache& c, int b) {
+            ++ahead;
+            // only a page that holds tokens is looked up (n <= table_cols * page, so `ahead` is then inside the table)
+            next = left > c.page - slot ? __ldg(c.table + (int64_t)b * c.table_cols + ahead) : -1;
+        }
+        __device__ __forceinline__ void begin(const RansKvCache& c, int b, int h, int n, int tile, int lane) {
+            const int t0 = tile * kTile;
+            ahead = t0 / c.page;
+            slot = t0 - ahead * c.page;
+            left = n - t0;
+            at_page(c, h, __ldg(c.table + (int64_t)b * c.table_cols + ahead), lane);
+            fetch_next(c, b);
+        }
+        __device__ __forceinline__ void advance(const RansKvCache& c, int b, int h, int lane) {
+            left -= kTile;
+            slot += kTile;
+            if (slot == c.page) {
+                slot = 0;
+                at_page(c, h, next, lane);
+                fetch_next(c, b);
+                return;
+            }
+            if (valid > 0) valid = min(left, kTile);
+            if constexpr (!kFp4) {
+                k += kTile * c.k_slot;
+                v += kTile * c.v_slot;
+            } else {
+                k += kTile * (D / 2);
+                v += kTile * (D / 2);
+                ks += kTile * kChunks;
+                vs += kTile * kChunks;
+            }
+        }
+    };
+
+    template <bool FULL>
+    static __device__ __forceinline__ void load_k(RawK& r, const RansKvCache& c, const Cursor& u, int lane) {
+        const int g = lane >> 2;
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        const int vrow[4] = {2 * q4, 2 * q4 + 1, 2 * q4 + 8, 2 * q4 + 9};
-        if constexpr (!kFp4) {
-            const char* kp = static_cast<const char*>(c.k) + pg * c.k_page + h * c.k_head + slot * c.k_slot + q4 * 16;
-            const char* vp = static_cast<const char*>(c.v) + pg * c.v_page + h * c.v_head + slot * c.v_slot + g * 16;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+            const bool in = FULL || g + 8 * i < u.valid;
+            if constexpr (!kFp4) {
+                const char* p = u.k + 8 * i * c.k_slot;
 #pragma unroll
-                for (int j = 0; j < kChunks; ++j)
-                    r.k[i][j] = g + 8 * i < r.valid ? load16(kp + (g + 8 * i) * c.k_slot + j * 64) : zero;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < D / 64; ++j)
-                    r.v[i][j] = vrow[i] < r.valid ? load16(vp + vrow[i] * c.v_slot + j * 128) : zero;
-        } else {
-            const int64_t row0 = (pg * c.kv_heads + h) * c.page + slot;
-            const uint8_t* kp = static_cast<const uint8_t*>(c.k) + row0 * (D / 2) + q4 * (D / 8);
-            const uint8_t* vp = static_cast<const uint8_t*>(c.v) + row0 * (D / 2) + g * (D / 16);
-            const uint8_t* ksp = c.k_scale + row0 * kChunks;
-            const uint8_t* vsp = c.v_scale + row0 * kChunks + (g & 1) * (D / 64);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = g + 8 * i;
-                const bool in = t < r.valid;
+                for (int j = 0; j < kChunks; ++j) r.k[i][j] = in ? load16(p + j * 64) : zero;
+            } else if constexpr (D == 64) {
+                const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(u.k + i * 8 * (D / 2))) : make_uint2(0, 0);
+                r.w[i][0] = w.x; r.w[i][1] = w.y;
+                r.s[i][0] = in ? __ldg(reinterpret_cast<const uint16_t*>(u.ks + i * 8 * kChunks)) : 0;
+            } else {
 #pragma unroll
                 for (int j = 0; j < kChunks; j += 4) {
-                    if constexpr (kChunks >= 4) {
-                        const uint4 w = in ? load16(kp + t * (D / 2) + j * 4) : zero;
-                        r.kw[i][j] = w.x; r.kw[i][j + 1] = w.y; r.kw[i][j + 2] = w.z; r.kw[i][j + 3] = w.w;
-                        r.ks[i][j / 4] = in ? __ldg(reinterpret_cast<const uint32_t*>(ksp + t * kChunks + j)) : 0;
-                    } else {
-                        const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(kp + t * (D / 2))) : make_uint2(0, 0);
-                        r.kw[i][0] = w.x; r.kw[i][1] = w.y;
-                        r.ks[i][0] = in ? __ldg(reinterpret_cast<const uint16_t*>(ksp + t * kChunks)) : 0;
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = vrow[i];
-                const bool in = t < r.valid;
-                if constexpr (D == 256) {
-                    const uint4 w = in ? load16(vp + t * (D / 2)) : zero;
-                    r.vw[i][0] = w.x; r.vw[i][1] = w.y; r.vw[i][2] = w.z; r.vw[i][3] = w.w;
-                    r.vs[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(vsp + t * kChunks)) : 0;
-                } else if constexpr (D == 128) {
-                    const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(vp + t * (D / 2))) : make_uint2(0, 0);
-                    r.vw[i][0] = w.x; r.vw[i][1] = w.y;
-                    r.vs[i] = in ? __ldg(reinterpret_cast<const uint16_t*>(vsp + t * kChunks)) : 0;
-                } else {
-                    r.vw[i][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(vp + t * (D / 2))) : 0;
-                    r.vs[i] = in ? __ldg(vsp + t * kChunks) : 0;
+                    const uint4 w = in ? load16(u.k + i * 8 * (D / 2) + j * 4) : zero;
+                    r.w[i][j] = w.x; r.w[i][j + 1] = w.y; r.w[i][j + 2] = w.z; r.w[i][j + 3] = w.w;
+                    r.s[i][j / 4] = in ? __ldg(reinterpret_cast<const uint32_t*>(u.ks + i * 8 * kChunks + j)) : 0;
                 }
             }
         }
     }
 
+    template <bool FULL>
+    static __device__ __forceinline__ void load_v(RawV& r, const RansKvCache& c, const char* v, const char* vs, int valid, int lane) {
+        const int q4 = lane & 3;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = (i & 1) + 8 * (i >> 1);
+            const bool in = FULL || 2 * q4 + row < valid;
+            if constexpr (!kFp4) {
+                const char* p = v + row * c.v_slot;
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) r.v[i][j] = in ? load16(p + j * 128) : zero;
+            } else {
+                const char* p = v + row * (D / 2);
+                const char* ps = vs + row * kChunks;
+                if constexpr (D == 256) {
+                    const uint4 w = in ? load16(p) : zero;
+                    r.w[i][0] = w.x; r.w[i][1] = w.y; r.w[i][2] = w.z; r.w[i][3] = w.w;
+                    r.s[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(ps)) : 0;
+                } else if constexpr (D == 128) {
+                    const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
+                    r.w[i][0] = w.x; r.w[i][1] = w.y;
+                    r.s[i] = in ? __ldg(reinterpret_cast<const uint16_t*>(ps)) : 0;
+                } else {
+                    r.w[i][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0;
+                    r.s[i] = in ? __ldg(reinterpret_cast<const uint8_t*>(ps)) : 0;
+                }
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void load_k(RawK& r, const RansKvCache& c, const Cursor& u, int lane) {
+        if (u.valid == kTile) load_k<true>(r, c, u, lane); else load_k<false>(r, c, u, lane);
+    }
+    static __device__ __forceinline__ void load_v(RawV& r, const RansKvCache& c, const char* v, const char* vs, int valid, int lane) {
+        if (valid == kTile) load_v<true>(r, c, v, vs, valid, lane); else load_v<false>(r, c, v, vs, valid, lane);
+    }
+
     struct State {
         float o[D / 16][NT][4];
         float m[NT][2], l[NT][2];
-        uint4 q[NT][kChunks];
         float qs[kFp4 ? NT : 1][2];      // 4-bit: the powers of two taken out of the two heads' queries, times scale
     };
 
-    // The queries of a head group, in the order of load()'s key values.  For 4-bit
+    // The queries of a head group, in the order of load_k()'s values, to the warp's place in shared memory
+    // ([NT][kChunks][32 lanes]; 16 registers less than keeping them, for four wide reads a tile).  For 4-bit
     // keys they become fp16: each head's largest value is first brought to
     // [2^14, 2^15) by a power of two, so that nothing overflows and what is lost is
     // below 2^-38 of it.
-    static __device__ __forceinline__ void begin(State& s, const AttendArgs& a, int b, int head0, int heads, int lane) {
+    static __device__ __forceinline__ void begin(State& s, uint4* qs, const AttendArgs& a, int b, int head0, int heads, int lane) {
         const int g = lane >> 2, q4 = lane & 3;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const bool in = t * 8 + g < heads;
             const char* qp = a.q + b * a.q_batch + (int64_t)(head0 + t * 8 + g) * a.q_head + q4 * 16;
             float top = 0.0f;
+            uint4 q[kChunks];
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) s.q[t][j] = in ? load16(qp + j * 64) : make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < kChunks; ++j) q[j] = in ? load16(qp + j * 64) : make_uint4(0, 0, 0, 0);
             if constexpr (kFp4) {
                 auto unpack = [&](uint32_t w) {
                     return a.q_half ? __half22float2(*reinterpret_cast<__half2*>(&w))
@@ -253,7 +320,7 @@ struct Attend {
                 for (int j = 0; j < kChunks; ++j)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const float2 f = unpack((&s.q[t][j].x)[w]);
+                        const float2 f = unpack((&q[j].x)[w]);
                         top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                     }
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
@@ -264,23 +331,25 @@ struct Attend {
                 for (int j = 0; j < kChunks; ++j)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const float2 f = unpack((&s.q[t][j].x)[w]);
-                        (&s.q[t][j].x)[w] = pack2<true>(f.x * down, f.y * down);
+                        const float2 f = unpack((&q[j].x)[w]);
+                        (&q[j].x)[w] = pack2<true>(f.x * down, f.y * down);
                     }
                 // a lane's scores are of heads 2 q4 and 2 q4 + 1
                 s.qs[t][0] = __shfl_sync(~0u, up, (2 * q4) * 4) * a.scale_log2;
                 s.qs[t][1] = __shfl_sync(~0u, up, (2 * q4 + 1) * 4) * a.scale_log2;
             }
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) qs[(t * kChunks + j) * 32 + lane] = q[j];
             s.m[t][0] = s.m[t][1] = -INFINITY;
             s.l[t][0] = s.l[t][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) s.o[i][t][0] = s.o[i][t][1] = s.o[i][t][2] = s.o[i][t][3] = 0.0f;
         }
+        __syncwarp();
     }
 
-    static __device__ __forceinline__ void step(State& s, const Raw& r, const AttendArgs& a, int64_t x, int lane) {
-        const int g = lane >> 2, q4 = lane & 3;
-        float sc[NT][4];
+    // S^T of a tile, scaled to powers of two.
+    static __device__ __forceinline__ void scores(const State& s, const uint4* qs, const RawK& r, const AttendArgs& a, float (&sc)[NT][4], int lane) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
         if constexpr (!kFp4) {
@@ -289,8 +358,9 @@ struct Attend {
                 const uint4 k0 = r.k[0][j], k1 = r.k[1][j];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    mma<kHalfK>(sc[t], k0.x, k1.x, k0.y, k1.y, s.q[t][j].x, s.q[t][j].y);
-                    mma<kHalfK>(sc[t], k0.z, k1.z, k0.w, k1.w, s.q[t][j].z, s.q[t][j].w);
+                    const uint4 q = qs[(t * kChunks + j) * 32 + lane];
+                    mma<KIND == RANS_KV_FP16>(sc[t], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
+                    mma<KIND == RANS_KV_FP16>(sc[t], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
                 }
             }
 #pragma unroll
@@ -303,16 +373,17 @@ struct Attend {
                 uint32_t w0[4], w1[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    w0[i] = e2m1_to_half2((r.kw[0][j] >> (8 * i)) & 255);
-                    w1[i] = e2m1_to_half2((r.kw[1][j] >> (8 * i)) & 255);
+                    w0[i] = e2m1_to_half2((r.w[0][j] >> (8 * i)) & 255);
+                    w1[i] = e2m1_to_half2((r.w[1][j] >> (8 * i)) & 255);
                 }
-                const float f0 = scale_of((r.ks[0][j / 4] >> (8 * (j % 4))) & 255);
-                const float f1 = scale_of((r.ks[1][j / 4] >> (8 * (j % 4))) & 255);
+                const float f0 = scale_of((r.s[0][j / 4] >> (8 * (j % 4))) & 255);
+                const float f1 = scale_of((r.s[1][j / 4] >> (8 * (j % 4))) & 255);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma<true>(d, w0[0], w1[0], w0[1], w1[1], s.q[t][j].x, s.q[t][j].y);
-                    mma<true>(d, w0[2], w1[2], w0[3], w1[3], s.q[t][j].z, s.q[t][j].w);
+                    const uint4 q = qs[(t * kChunks + j) * 32 + lane];
+                    mma<true>(d, w0[0], w1[0], w0[1], w1[1], q.x, q.y);
+                    mma<true>(d, w0[2], w1[2], w0[3], w1[3], q.z, q.w);
                     sc[t][0] = fmaf(d[0], f0, sc[t][0]);
                     sc[t][1] = fmaf(d[1], f0, sc[t][1]);
                     sc[t][2] = fmaf(d[2], f1, sc[t][2]);
@@ -325,11 +396,19 @@ struct Attend {
                 sc[t][2] *= s.qs[t][0]; sc[t][3] *= s.qs[t][1];
             }
         }
+    }
+
+    // The softmax's part of a tile of `valid` tokens: scores become P^T's operands, the maximum, the sum and O follow.
+    static __device__ __forceinline__ void probabilities(State& s, float (&sc)[NT][4], uint32_t (&pb)[NT][2], const AttendArgs& a,
+                                                         int64_t x, int valid, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
         bool raise_max = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (g >= r.valid) sc[t][0] = sc[t][1] = -INFINITY;
-            if (g + 8 >= r.valid) sc[t][2] = sc[t][3] = -INFINITY;
+            if (valid < kTile) {
+                if (g >= valid) sc[t][0] = sc[t][1] = -INFINITY;
+                if (g + 8 >= valid) sc[t][2] = sc[t][3] = -INFINITY;
+            }
             if (a.weigh && x < a.score_tiles) {
                 float* p = a.scores + (x * kTile + g) * HP + t * 8 + 2 * q4;
                 *reinterpret_cast<float2*>(p) = make_float2(sc[t][0], sc[t][1]);
@@ -357,7 +436,6 @@ struct Attend {
                     }
                 }
         }
-        uint32_t pb[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float m0 = s.m[t][0] == -INFINITY ? 0.0f : s.m[t][0], m1 = s.m[t][1] == -INFINITY ? 0.0f : s.m[t][1];
@@ -368,6 +446,10 @@ struct Attend {
             pb[t][0] = transpose8x8(pack2<kHalfV>(p0, p1));
             pb[t][1] = transpose8x8(pack2<kHalfV>(p2, p3));
         }
+    }
+
+    // O^T += V^T P^T.
+    static __device__ __forceinline__ void accumulate(State& s, const RawV& r, const uint32_t (&pb)[NT][2]) {
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             if constexpr (!kFp4) {
@@ -383,10 +465,10 @@ struct Attend {
                     for (int t = 0; t < NT; ++t) mma<kHalfV>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
                 }
             } else {
-                const uint32_t lo01 = __byte_perm(r.vw[0][j], r.vw[1][j], 0x5410), hi01 = __byte_perm(r.vw[0][j], r.vw[1][j], 0x7632);
-                const uint32_t lo23 = __byte_perm(r.vw[2][j], r.vw[3][j], 0x5410), hi23 = __byte_perm(r.vw[2][j], r.vw[3][j], 0x7632);
-                const uint32_t f01 = factor2((r.vs[0] >> (8 * j)) & 255, (r.vs[1] >> (8 * j)) & 255);
-                const uint32_t f23 = factor2((r.vs[2] >> (8 * j)) & 255, (r.vs[3] >> (8 * j)) & 255);
+                const uint32_t lo01 = __byte_perm(r.w[0][j], r.w[1][j], 0x5410), hi01 = __byte_perm(r.w[0][j], r.w[1][j], 0x7632);
+                const uint32_t lo23 = __byte_perm(r.w[2][j], r.w[3][j], 0x5410), hi23 = __byte_perm(r.w[2][j], r.w[3][j], 0x7632);
+                const uint32_t f01 = factor2((r.s[0] >> (8 * j)) & 255, (r.s[1] >> (8 * j)) & 255);
+                const uint32_t f23 = factor2((r.s[2] >> (8 * j)) & 255, (r.s[3] >> (8 * j)) & 255);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     auto value = [&](uint32_t w, uint32_t f) {
@@ -456,7 +538,7 @@ struct Attend {
             }
     }
 
-    static __device__ __forceinline__ void write_part(const State& s, Smem& sm, int slot, int lane) {
+    static __device__ __forceinline__ void write_part(const State& s, Part& part, int lane) {
         const int g = lane >> 2, q4 = lane & 3;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -467,14 +549,52 @@ struct Attend {
                 for (int j = 0; j < D / 64; ++j)
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        *reinterpret_cast<float4*>(&sm.o[slot][head][first_d(j, g) + 4 * i]) =
+                        *reinterpret_cast<float4*>(&part.o[head][first_d(j, g) + 4 * i]) =
                             make_float4(value_of(s, j, t, e, 4 * i), value_of(s, j, t, e, 4 * i + 1),
                                         value_of(s, j, t, e, 4 * i + 2), value_of(s, j, t, e, 4 * i + 3));
-                if (g == 0) {
-                    sm.m[slot][head] = s.m[t][e];
-                    sm.l[slot][head] = s.l[t][e];
+                if (g == 0) part.ml[head] = make_float2(s.m[t][e], s.l[t][e]);
+            }
+    }
+
+    // Joins four values of one head over n parts, in their order, eight parts' loads at once.  Every column's thread works
+    // out the factors for itself: that costs a few exponentials, and no barrier and no second trip to memory.
+    template <bool SHARED, class PartAt>
+    static __device__ __forceinline__ void join(PartAt part_at, int n, int head, int d, float4& o, float& top, float& l) {
+        constexpr int kAtOnce = 8;
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        top = -INFINITY;
+        l = 0.0f;
+        for (int k = 0; k < n; k += kAtOnce) {
+            float4 y[kAtOnce];
+            float2 ml[kAtOnce];
+            float m = top;
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                ml[e] = make_float2(-INFINITY, 0.0f);
+                if (k + e < n) {
+                    const Part* p = part_at(k + e);
+                    if constexpr (SHARED) {
+                        ml[e] = p->ml[head];
+                        y[e] = *reinterpret_cast<const float4*>(&p->o[head][d]);
+                    } else {
+                        ml[e] = __ldcg(&p->ml[head]);
+                        y[e] = __ldcg(reinterpret_cast<const float4*>(&p->o[head][d]));
+                    }
                 }
             }
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) m = fmaxf(m, ml[e].x);
+            const float down = join_factor(top, m);
+            o.x *= down; o.y *= down; o.z *= down; o.w *= down; l *= down;
+            top = m;
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const float f = join_factor(ml[e].x, m);
+                o.x = fmaf(y[e].x, f, o.x); o.y = fmaf(y[e].y, f, o.y); o.z = fmaf(y[e].z, f, o.z); o.w = fmaf(y[e].w, f, o.w);
+                l = fmaf(ml[e].y, f, l);
+            }
+        }
     }
 
     static __device__ __forceinline__ void store_joined(const AttendArgs& a, int b, int head, int d, float4 o, float m, float l) {
@@ -487,10 +607,24 @@ struct Attend {
     }
 };
 
-__device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
+// Adds one and returns what was there: the parts written before the barrier in front of it are seen by whoever finds
+// the last count, and that one sees everybody's.
+__device__ __forceinline__ int count_up(int* p) {
+    int old;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+    return old;
+}
+
+// A (sequence, kv head, part of its group) in one word: at most 2048, 1024 and 16 of them.
+struct Group {
+    int b, h, sub;
+    __device__ __forceinline__ int pack() const { return (b << 14) | (h << 4) | sub; }
+    static __device__ __forceinline__ Group of(int tag) { return {tag >> 14, (tag >> 4) & 1023, tag & 15}; }
+};
 
 template <int KIND, int D, int NT>
-__global__ void __launch_bounds__(Attend<KIND, D, NT>::kWarps * 32, Attend<KIND, D, NT>::kBlocksPerSm)
+__global__ void __launch_bounds__(Attend<KIND, D, NT>::kWarps * 32, 1)
 attend_kernel(const __grid_constant__ AttendArgs a) {
     using A = Attend<KIND, D, NT>;
     constexpr int HP = A::HP, W = A::kWarps, kThreads = W * 32;
@@ -498,13 +632,13 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     typename A::Smem& sm = *reinterpret_cast<typename A::Smem*>(smem_raw);
     const RansKvCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int segs = c.kv_heads * a.subs;               // (kv head, part of its group) of one sequence
+    const int segs = c.kv_heads * a.subs;               // groups of one sequence
 
     // Tiles in front of each sequence.
     {
         const int per = (c.batch + kThreads - 1) / kThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
         int sum = 0;
-        for (int b = b0; b < b1; ++b) sum += (checked_length(c, b) + kTile - 1) / kTile * segs;
+        for (int b = b0; b < b1; ++b) sum += (checked_length(c, b) + kTile - 1) / kTile;
         int inc = sum;
 #pragma unroll
         for (int i = 1; i < 32; i *= 2) {
@@ -512,19 +646,18 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             if (lane >= i) inc += y;
         }
         if (lane == 31) sm.warp_sum[warp] = inc;
-        if (lane < 2) sm.tag[warp * 2 + lane] = -1;
+        if (lane < 2) sm.tag[lane * W + warp] = -1;
         __syncthreads();
         int at = inc - sum;
         for (int w = 0; w < warp; ++w) at += sm.warp_sum[w];
         for (int b = b0; b < b1; ++b) {
             sm.pre[b] = at;
-            at += (checked_length(c, b) + kTile - 1) / kTile * segs;
+            at += (checked_length(c, b) + kTile - 1) / kTile;
         }
         if (b1 == c.batch && b0 < b1) sm.pre[c.batch] = at;
         __syncthreads();
     }
-    const int total = sm.pre[c.batch];
-    auto tiles_of = [&](int b) { return (sm.pre[b + 1] - sm.pre[b]) / segs; };
+    const int total = sm.pre[c.batch] * segs;
 
     // Sequences without tokens.
     for (int b = blockIdx.x; b < c.batch; b += gridDim.x)
@@ -534,136 +667,169 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                 if (i < a.heads && a.log_sum != nullptr) a.log_sum[(int64_t)b * a.heads + i] = -INFINITY;
             }
 
+    static_assert(kThreads >= kGrid, "a thread for every block");
+    // Equal runs of tiles: per block, and in it per warp.
     const int blocks = min((int)gridDim.x, (total + W - 1) / W);       // each of their warps has a tile
     if ((int)blockIdx.x >= blocks) return;
-    const int x0 = (int)((int64_t)total * blockIdx.x / blocks), x1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
-    int x = x0 + (int)((int64_t)(x1 - x0) * warp / W);
-    const int xe = x0 + (int)((int64_t)(x1 - x0) * (warp + 1) / W);
+    const int per_block = total / blocks, longer = total - per_block * blocks;       // the first `longer` have one more
+    auto first_of = [&](int block) { return per_block * block + min(block, longer); };
+    const int x0 = first_of(blockIdx.x), x1 = first_of(blockIdx.x + 1);
+    const int per_warp = (x1 - x0) / W, warps_longer = x1 - x0 - per_warp * W;
+    int x = x0 + per_warp * warp + min(warp, warps_longer);
+    const int xe = x + per_warp + (warp < warps_longer ? 1 : 0);
+    auto heads_of = [&](const Group& s) { return min(a.sub_heads, a.group - s.sub * a.sub_heads); };
+    auto head0_of = [&](const Group& s) { return s.h * a.group + s.sub * a.sub_heads; };
 
     if (x < xe) {
-        int lo = 0, hi = c.batch;                       // the sequence of tile x: pre[lo] <= x < pre[lo + 1]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (sm.pre[mid] <= x) lo = mid; else hi = mid;
+        Group s;
+        int nt, tile;
+        {
+            int lo = 0, hi = c.batch;                   // the sequence of tile x: pre[lo] * segs <= x < pre[lo + 1] * segs
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (sm.pre[mid] * segs <= x) lo = mid; else hi = mid;
+            }
+            nt = sm.pre[lo + 1] - sm.pre[lo];
+            const int in = x - sm.pre[lo] * segs, seg = in / nt;
+            tile = in - seg * nt;
+            s.b = lo;
+            s.h = seg / a.subs;
+            s.sub = seg - s.h * a.subs;
         }
-        int b = lo, nt = tiles_of(b), seg = (x - sm.pre[b]) / nt, tile = (x - sm.pre[b]) - seg * nt, parts = 0;
-        typename A::State s;
-        while (x < xe) {
-            const int end = min(tile + (xe - x), nt);
-            const int h = seg / a.subs, sub = seg - h * a.subs;
-            const int head0 = h * a.group + sub * a.sub_heads, heads = min(a.sub_heads, a.group - sub * a.sub_heads);
-            const int n = checked_length(c, b);
-            const bool whole = tile == 0 && end == nt;
-            A::begin(s, a, b, head0, heads, lane);
-            for (; tile < end; ++tile, ++x) {
-                typename A::Raw r;
-                A::load(r, a, b, h, n, tile, lane);
-                A::step(s, r, a, x, lane);
-            }
-            A::reduce_sum(s);
-            if (whole) {
-                A::write_out(s, a, b, head0, heads, lane);
-            } else {
-                A::write_part(s, sm, warp * 2 + parts, lane);
-                if (lane == 0) sm.tag[warp * 2 + parts] = b * segs + seg;
-                ++parts;
-            }
-            tile = 0;
-            if (++seg == segs) {
-                seg = 0;
-                do ++b; while (b < c.batch && sm.pre[b + 1] == sm.pre[b]);
-                if (b < c.batch) nt = tiles_of(b);
-            }
-        }
-    }
-    __syncthreads();
-
-    // Join the warps' parts of each (sequence, head group); what this block has not all of goes to `part`.
-    constexpr int kVec = HP * (D / 4);
-    int open[2] = {-1, -1};
-    for (int i0 = 0; i0 < W * 2;) {
-        const int tag = sm.tag[i0];
-        if (tag < 0) { ++i0; continue; }
-        int i1 = i0 + 1;
-        while (i1 < W * 2 && (sm.tag[i1] == tag || sm.tag[i1] < 0)) ++i1;
-        const int b = tag / segs, seg = tag - b * segs, nt = tiles_of(b), start = sm.pre[b] + seg * nt;
-        const int h = seg / a.subs, sub = seg - h * a.subs;
-        const int head0 = h * a.group + sub * a.sub_heads, heads = min(a.sub_heads, a.group - sub * a.sub_heads);
-        const bool whole = start >= x0 && start + nt <= x1;
-        const int slot = start <= x0 ? 0 : 1;
-        if (!whole) open[slot] = tag;
-        float* part = a.part + (int64_t)(blockIdx.x * 2 + slot) * HP * (D + 2);
-        for (int v = tid; v < kVec; v += kThreads) {
-            const int head = v / (D / 4), d = v % (D / 4) * 4;
-            if (head >= heads) break;
-            float top = -INFINITY;
-            for (int i = i0; i < i1; ++i)
-                if (sm.tag[i] >= 0) top = fmaxf(top, sm.m[i][head]);
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float l = 0.0f;
-            for (int i = i0; i < i1; ++i) {
-                if (sm.tag[i] < 0) continue;
-                const float f = join_factor(sm.m[i][head], top);
-                const float4 y = *reinterpret_cast<const float4*>(&sm.o[i][head][d]);
-                o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
-                l = fmaf(sm.l[i][head], f, l);
-            }
-            if (whole) {
-                A::store_joined(a, b, head0 + head, d, o, top, l);
-            } else {
-                __stcg(reinterpret_cast<float4*>(part + head * D + d), o);
-                if (d == 0) {
-                    __stcg(part + HP * D + head * 2, top);
-                    __stcg(part + HP * D + head * 2 + 1, l);
+        // A warp's second part is written when it is done, so until then its queries live there.
+        uint4* qs = reinterpret_cast<uint4*>(&sm.part[W + warp]);
+        static_assert(sizeof(typename A::Part) >= NT * A::kChunks * 32 * sizeof(uint4), "room for the queries");
+        typename A::State st;
+        typename A::Cursor u;
+        typename A::RawK rk;
+        typename A::RawV rv;
+        int flushed = 0, valid = 0;
+        bool have = false, whole = false, fresh = true;
+        // Keys of the next tile are on their way while this tile's softmax and values are worked on, and values while the
+        // next scores are: the same registers, refilled as soon as their contents are used.
+        while (true) {
+            float sc[NT][4];
+            uint32_t pb[NT][2];
+            bool more = true, ends = false;
+            const Group now = s;
+            if (have) {
+                A::scores(st, qs, rk, a, sc, lane);
+                more = x + 1 < xe;
+                ends = ++tile == nt;
+                valid = u.valid;
+                fresh = ends;
+                if (ends && more) {
+                    tile = 0;
+                    if (++s.sub == a.subs) {
+                        s.sub = 0;
+                        if (++s.h == c.kv_heads) {
+                            s.h = 0;
+                            do ++s.b; while (sm.pre[s.b + 1] == sm.pre[s.b]);
+                            nt = sm.pre[s.b + 1] - sm.pre[s.b];
+                        }
+                    }
                 }
             }
+            if (more) {
+                if (fresh) u.begin(c, s.b, s.h, checked_length(c, s.b), tile, lane); else u.advance(c, s.b, s.h, lane);
+                A::load_k(rk, c, u, lane);
+            }
+            if (have) {
+                A::probabilities(st, sc, pb, a, x, valid, lane);
+                A::accumulate(st, rv, pb);
+                ++x;
+                if (ends || !more) {
+                    A::reduce_sum(st);
+                    __syncwarp();
+                    if (whole && ends) {
+                        A::write_out(st, a, now.b, head0_of(now), heads_of(now), lane);
+                    } else {
+                        A::write_part(st, sm.part[flushed * W + warp], lane);
+                        if (lane == 0) sm.tag[flushed * W + warp] = now.pack();
+                        ++flushed;
+                    }
+                }
+            }
+            if (!more) break;
+            if (fresh) {
+                whole = tile == 0;
+                A::begin(st, qs, a, s.b, head0_of(s), heads_of(s), lane);
+                fresh = false;
+            }
+            A::load_v(rv, c, u.v, u.vs, u.valid, lane);
+            have = true;
         }
-        i0 = i1;
     }
-
-    // The last block of a (sequence, head group) joins the blocks' parts.
-    __threadfence();
     __syncthreads();
-    auto block_of = [&](int tile) { return (int)((((int64_t)tile + 1) * blocks - 1) / total); };
-    if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            sm.last[i] = 0;
-            if (open[i] < 0) continue;
-            const int b = open[i] / segs, seg = open[i] - b * segs, nt = tiles_of(b), start = sm.pre[b] + seg * nt;
-            const int splits = block_of(start + nt - 1) - block_of(start) + 1;
-            if (atomicAdd(a.counter + open[i], 1) == splits - 1) {
-                a.counter[open[i]] = 0;
-                sm.last[i] = 1;
+
+    // Join the warps' parts group by group (each warp finds the groups for itself); what the block has not all of goes to
+    // the workspace.
+    static_assert(W * 2 <= 32, "one lane per part");
+    constexpr int kVec = HP * (D / 4);
+    typename A::Part* parts = reinterpret_cast<typename A::Part*>(a.part);
+    int open0 = -1, open1 = -1;                          // groups that the block has only some of: its first, its last
+    const int my_tag = lane < W * 2 ? sm.tag[lane] : -1;
+    for (unsigned left = __ballot_sync(~0u, my_tag >= 0); left != 0;) {
+        const int tag = __shfl_sync(~0u, my_tag, __ffs(left) - 1);
+        const unsigned run = __ballot_sync(~0u, my_tag == tag);
+        left &= ~run;
+        const Group s = Group::of(tag);
+        const int nt = sm.pre[s.b + 1] - sm.pre[s.b], start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * nt;
+        const bool whole = start >= x0 && start + nt <= x1;
+        const int slot = start <= x0 ? 0 : 1, heads = heads_of(s);
+        if (!whole) {
+            if (slot == 0) open0 = tag; else open1 = tag;
+            // which blocks share the group: every thread looks at one block (no division)
+            if (tid < blocks) {
+                const int f0 = first_of(tid), f1 = first_of(tid + 1);
+                if (f0 <= start && start < f1) sm.first_block[slot] = tid;
+                if (f0 < start + nt && start + nt <= f1) sm.last_block[slot] = tid;
             }
         }
-        __threadfence();
-    }
-    __syncthreads();
-    for (int i = 0; i < 2; ++i) {
-        if (!sm.last[i]) continue;
-        const int b = open[i] / segs, seg = open[i] - b * segs, nt = tiles_of(b), start = sm.pre[b] + seg * nt;
-        const int h = seg / a.subs, sub = seg - h * a.subs;
-        const int head0 = h * a.group + sub * a.sub_heads, heads = min(a.sub_heads, a.group - sub * a.sub_heads);
-        const int c0 = block_of(start), c1 = block_of(start + nt - 1);
-        const int slot0 = (int64_t)total * c0 / blocks >= start ? 0 : 1;     // only the first block's part may be its second
-        auto part_of = [&](int k) { return a.part + (int64_t)(k * 2 + (k == c0 ? slot0 : 0)) * HP * (D + 2); };
         for (int v = tid; v < kVec; v += kThreads) {
             const int head = v / (D / 4), d = v % (D / 4) * 4;
             if (head >= heads) break;
-            float top = -INFINITY;
-            for (int k = c0; k <= c1; ++k) top = fmaxf(top, __ldcg(part_of(k) + HP * D + head * 2));
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float l = 0.0f;
-#pragma unroll 4
-            for (int k = c0; k <= c1; ++k) {
-                const float* p = part_of(k);
-                const float f = join_factor(__ldcg(p + HP * D + head * 2), top);
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(p + head * D + d));
-                o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
-                l = fmaf(__ldcg(p + HP * D + head * 2 + 1), f, l);
+            float4 o;
+            float top, l;
+            unsigned rest = run;
+            A::template join<true>([&](int) { const int e = __ffs(rest) - 1; rest &= rest - 1; return &sm.part[e]; }, __popc(run), head, d, o, top, l);
+            if (whole) {
+                A::store_joined(a, s.b, head0_of(s) + head, d, o, top, l);
+            } else {
+                typename A::Part* mine = parts + blockIdx.x * 2 + slot;
+                __stcg(reinterpret_cast<float4*>(&mine->o[head][d]), o);
+                if (d == 0) __stcg(&mine->ml[head], make_float2(top, l));
             }
-            A::store_joined(a, b, head0 + head, d, o, top, l);
         }
+    }
+
+    // The last block of a group to get here joins the blocks' parts.
+    if (open0 < 0 && open1 < 0) return;
+    __syncthreads();
+    if (tid < 2) {
+        const int tag = tid == 0 ? open0 : open1;
+        bool last = false;
+        if (tag >= 0) {
+            const Group s = Group::of(tag);
+            int* counter = a.counter + s.b * segs + s.h * a.subs + s.sub;
+            last = count_up(counter) == sm.last_block[tid] - sm.first_block[tid];
+            if (last) *counter = 0;
+        }
+        sm.last[tid] = last;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int v = tid; v < 2 * kVec; v += kThreads) {
+        const int i = v / kVec, head = v % kVec / (D / 4), d = v % (D / 4) * 4;
+        if (!sm.last[i]) continue;
+        const Group s = Group::of(i == 0 ? open0 : open1);
+        if (head >= heads_of(s)) continue;
+        const int nt = sm.pre[s.b + 1] - sm.pre[s.b], start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * nt;
+        const int c0 = sm.first_block[i], second = first_of(c0) == start ? 0 : 1;    // only a group's first block has it as its second
+        float4 o;
+        float top, l;
+        A::template join<false>([&](int k) { return parts + (c0 + k) * 2 + (k == 0 ? second : 0); }, sm.last_block[i] - c0 + 1, head, d, o, top, l);
+        A::store_joined(a, s.b, head0_of(s) + head, d, o, top, l);
     }
 }
 
@@ -728,8 +894,6 @@ struct Plan {
     int64_t counter, stats, part, scores, bytes, score_tiles;
 };
 
-constexpr int kGrid = kSms * 2;
-
 bool make_plan(const RansKvCache& c, int heads, int weigh, Plan& p) {
     if (heads < 1 || heads % c.kv_heads != 0) return false;
     const int group = heads / c.kv_heads, most = c.dim == 256 ? 8 : 16;
@@ -737,11 +901,13 @@ bool make_plan(const RansKvCache& c, int heads, int weigh, Plan& p) {
     if (p.subs > kMaxSubgroups) return false;
     p.sub_heads = (group + p.subs - 1) / p.subs;
     p.nt = p.sub_heads > 8 ? 2 : 1;
+    // tiles are counted in 32 bits
+    if (((int64_t)c.table_cols * c.page / kTile + 1) * c.batch * c.kv_heads * p.subs > 0x7fffffff) return false;
     auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
     p.counter = 256;
     p.stats = counter_bytes(c);
     p.part = p.stats + up((int64_t)c.batch * heads * 8);
-    p.scores = p.part + up((int64_t)kGrid * 2 * p.nt * 8 * (c.dim + 2) * 4);
+    p.scores = p.part + up((int64_t)kGrid * 2 * p.nt * 8 * (c.dim + 4 + 2) * 4);
     // every token of every page, and a started tile for each sequence
     p.score_tiles = weigh ? ((int64_t)c.pages * c.page / kTile + c.batch) * c.kv_heads * p.subs : 0;
     p.bytes = p.scores + up(p.score_tiles * kTile * p.nt * 8 * 4);

@@ -47,7 +47,7 @@ inline int check_cache(const RansKvCache* c) {
     if (c == nullptr) return -2;
     if (c->kind != RANS_KV_BF16 && c->kind != RANS_KV_FP16 && c->kind != RANS_KV_MXFP4) return -1;
     if (c->dim != 64 && c->dim != 128 && c->dim != 256) return -1;
-    if (c->pages < 1 || c->page < 16 || c->page % 16 != 0 || c->page > (1 << 20) || c->kv_heads < 1 || c->batch < 1 ||
+    if (c->pages < 1 || c->page < 16 || c->page % 16 != 0 || c->page > (1 << 20) || c->kv_heads < 1 || c->kv_heads > 1024 || c->batch < 1 ||
         c->batch > RANS_KV_MAX_BATCH || (int64_t)c->batch * c->kv_heads > 65535 || c->table_cols < 1 || c->reserved != 0)
         return -2;
     if ((int64_t)c->table_cols * c->page > (int64_t)1 << 30) return -2;
