@@ -26,6 +26,7 @@
 // shared memory, and the last block to finish a (sequence, kv head) joins the
 // blocks' parts (always in the order of the tiles, so results do not depend on
 // which block that is).
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -43,6 +44,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 16;
 constexpr int kGrid = kSms;
+// A group's first tile waits for its page number and queries, and its end is written out: in the shares of work it
+// counts as this many tiles more (places without a tile behind the group's last one).
+constexpr int kStart = 2;
 // The maximum is only raised when a score passes it by this much (in powers of
 // two): probabilities then stay below 2^8, harmless in bf16, fp16 and fp32.
 constexpr float kSlack = 8.0f;
@@ -153,7 +157,7 @@ struct Attend {
         int tag[kWarps * 2];                 // the group of each part
         int first_block[2], last_block[2], last[2];      // of the block's first and last group, if it has only some of it
         int warp_sum[kWarps];
-        int pre[RANS_KV_MAX_BATCH + 1];      // tiles of one head in front of each sequence
+        int pre[RANS_KV_MAX_BATCH + 1];      // places of one head in front of each sequence
     };
 
     // One tile's rows as they come from memory.
@@ -608,6 +612,9 @@ struct Attend {
 };
 
 
+// Places of one head's group of a sequence of n tokens in the shares of work.
+__device__ __forceinline__ int places_of(int n) { return n > 0 ? (n + kTile - 1) / kTile + kStart : 0; }
+
 // Adds one and returns what was there: the parts written before the barrier in front of it are seen by whoever finds
 // the last count, and that one sees everybody's.
 __device__ __forceinline__ int count_up(int* p) {
@@ -634,11 +641,11 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int segs = c.kv_heads * a.subs;               // groups of one sequence
 
-    // Tiles in front of each sequence.
+    // Places in front of each sequence.
     {
         const int per = (c.batch + kThreads - 1) / kThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
         int sum = 0;
-        for (int b = b0; b < b1; ++b) sum += (checked_length(c, b) + kTile - 1) / kTile;
+        for (int b = b0; b < b1; ++b) sum += places_of(checked_length(c, b));
         int inc = sum;
 #pragma unroll
         for (int i = 1; i < 32; i *= 2) {
@@ -652,7 +659,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         for (int w = 0; w < warp; ++w) at += sm.warp_sum[w];
         for (int b = b0; b < b1; ++b) {
             sm.pre[b] = at;
-            at += (checked_length(c, b) + kTile - 1) / kTile;
+            at += places_of(checked_length(c, b));
         }
         if (b1 == c.batch && b0 < b1) sm.pre[c.batch] = at;
         __syncthreads();
@@ -668,7 +675,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             }
 
     static_assert(kThreads >= kGrid, "a thread for every block");
-    // Equal runs of tiles: per block, and in it per warp.
+    // Equal runs of places: per block, and in it per warp.
     const int blocks = min((int)gridDim.x, (total + W - 1) / W);       // each of their warps has a tile
     if ((int)blockIdx.x >= blocks) return;
     const int per_block = total / blocks, longer = total - per_block * blocks;       // the first `longer` have one more
@@ -677,25 +684,39 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     const int per_warp = (x1 - x0) / W, warps_longer = x1 - x0 - per_warp * W;
     int x = x0 + per_warp * warp + min(warp, warps_longer);
     const int xe = x + per_warp + (warp < warps_longer ? 1 : 0);
+    auto tiles_of = [&](int b) { return sm.pre[b + 1] - sm.pre[b] - kStart; };
     auto heads_of = [&](const Group& s) { return min(a.sub_heads, a.group - s.sub * a.sub_heads); };
     auto head0_of = [&](const Group& s) { return s.h * a.group + s.sub * a.sub_heads; };
 
+    Group s{};
+    int nt = 0, tile = 0;
+    auto next_group = [&]() {
+        tile = 0;
+        if (++s.sub < a.subs) return;
+        s.sub = 0;
+        if (++s.h < c.kv_heads) return;
+        s.h = 0;
+        do ++s.b; while (s.b < c.batch && sm.pre[s.b + 1] == sm.pre[s.b]);
+        if (s.b < c.batch) nt = tiles_of(s.b);
+    };
     if (x < xe) {
-        Group s;
-        int nt, tile;
-        {
-            int lo = 0, hi = c.batch;                   // the sequence of tile x: pre[lo] * segs <= x < pre[lo + 1] * segs
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (sm.pre[mid] * segs <= x) lo = mid; else hi = mid;
-            }
-            nt = sm.pre[lo + 1] - sm.pre[lo];
-            const int in = x - sm.pre[lo] * segs, seg = in / nt;
-            tile = in - seg * nt;
-            s.b = lo;
-            s.h = seg / a.subs;
-            s.sub = seg - s.h * a.subs;
+        int lo = 0, hi = c.batch;                       // the sequence of place x: pre[lo] * segs <= x < pre[lo + 1] * segs
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (sm.pre[mid] * segs <= x) lo = mid; else hi = mid;
         }
+        nt = tiles_of(lo);
+        const int in = x - sm.pre[lo] * segs, seg = in / (nt + kStart);
+        tile = in - seg * (nt + kStart);
+        s.b = lo;
+        s.h = seg / a.subs;
+        s.sub = seg - s.h * a.subs;
+        if (tile >= nt) {                               // behind a group's last tile
+            x += nt + kStart - tile;
+            next_group();
+        }
+    }
+    if (x < xe) {
         // A warp's second part is written when it is done, so until then its queries live there.
         uint4* qs = reinterpret_cast<uint4*>(&sm.part[W + warp]);
         static_assert(sizeof(typename A::Part) >= NT * A::kChunks * 32 * sizeof(uint4), "room for the queries");
@@ -703,7 +724,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         typename A::Cursor u;
         typename A::RawK rk;
         typename A::RawV rv;
-        int flushed = 0, valid = 0;
+        int flushed = 0, valid = 0, next = 0;
         bool have = false, whole = false, fresh = true;
         // Keys of the next tile are on their way while this tile's softmax and values are worked on, and values while the
         // next scores are: the same registers, refilled as soon as their contents are used.
@@ -714,21 +735,12 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             const Group now = s;
             if (have) {
                 A::scores(st, qs, rk, a, sc, lane);
-                more = x + 1 < xe;
                 ends = ++tile == nt;
+                next = x + 1 + (ends ? kStart : 0);
+                more = next < xe;
                 valid = u.valid;
                 fresh = ends;
-                if (ends && more) {
-                    tile = 0;
-                    if (++s.sub == a.subs) {
-                        s.sub = 0;
-                        if (++s.h == c.kv_heads) {
-                            s.h = 0;
-                            do ++s.b; while (sm.pre[s.b + 1] == sm.pre[s.b]);
-                            nt = sm.pre[s.b + 1] - sm.pre[s.b];
-                        }
-                    }
-                }
+                if (ends && more) next_group();
             }
             if (more) {
                 if (fresh) u.begin(c, s.b, s.h, checked_length(c, s.b), tile, lane); else u.advance(c, s.b, s.h, lane);
@@ -737,7 +749,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             if (have) {
                 A::probabilities(st, sc, pb, a, x, valid, lane);
                 A::accumulate(st, rv, pb);
-                ++x;
+                x = next;
                 if (ends || !more) {
                     A::reduce_sum(st);
                     __syncwarp();
@@ -774,7 +786,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         const unsigned run = __ballot_sync(~0u, my_tag == tag);
         left &= ~run;
         const Group s = Group::of(tag);
-        const int nt = sm.pre[s.b + 1] - sm.pre[s.b], start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * nt;
+        const int nt = tiles_of(s.b), start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * (nt + kStart);
         const bool whole = start >= x0 && start + nt <= x1;
         const int slot = start <= x0 ? 0 : 1, heads = heads_of(s);
         if (!whole) {
@@ -824,7 +836,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         if (!sm.last[i]) continue;
         const Group s = Group::of(i == 0 ? open0 : open1);
         if (head >= heads_of(s)) continue;
-        const int nt = sm.pre[s.b + 1] - sm.pre[s.b], start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * nt;
+        const int nt = tiles_of(s.b), start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * (nt + kStart);
         const int c0 = sm.first_block[i], second = first_of(c0) == start ? 0 : 1;    // only a group's first block has it as its second
         float4 o;
         float top, l;
@@ -843,7 +855,7 @@ __global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (c.batch + kWeighThreads - 1) / kWeighThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += (checked_length(c, b) + kTile - 1) / kTile;
+    for (int b = b0; b < b1; ++b) sum += places_of(checked_length(c, b));
     int inc = sum;
 #pragma unroll
     for (int i = 1; i < 32; i *= 2) {
@@ -856,14 +868,14 @@ __global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_const
     for (int w = 0; w < warp; ++w) at += warp_sum[w];
     for (int b = b0; b < b1; ++b) {
         pre[b] = at;
-        at += (checked_length(c, b) + kTile - 1) / kTile;
+        at += places_of(checked_length(c, b));
     }
     if (b1 == c.batch && b0 < b1) pre[c.batch] = at;
     __syncthreads();
-    const int total = pre[c.batch];                     // tiles of one head of every sequence
+    const int total = pre[c.batch];                     // places of one head of every sequence, as in attend_kernel
     const int64_t all = (int64_t)total * c.kv_heads * kTile;
     for (int64_t i = (int64_t)blockIdx.x * kWeighThreads + tid; i < all; i += (int64_t)gridDim.x * kWeighThreads) {
-        const int64_t xt = i / kTile;                   // (sequence, kv head, tile)
+        const int64_t xt = i / kTile;                   // (sequence, kv head, place)
         int lo = 0, hi = c.batch;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
@@ -901,15 +913,15 @@ bool make_plan(const RansKvCache& c, int heads, int weigh, Plan& p) {
     if (p.subs > kMaxSubgroups) return false;
     p.sub_heads = (group + p.subs - 1) / p.subs;
     p.nt = p.sub_heads > 8 ? 2 : 1;
-    // tiles are counted in 32 bits
-    if (((int64_t)c.table_cols * c.page / kTile + 1) * c.batch * c.kv_heads * p.subs > 0x7fffffff) return false;
+    // places are counted in 32 bits
+    if (((int64_t)c.table_cols * c.page / kTile + kStart) * c.batch * c.kv_heads * p.subs > 0x7fffffff) return false;
     auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
     p.counter = 256;
     p.stats = counter_bytes(c);
     p.part = p.stats + up((int64_t)c.batch * heads * 8);
     p.scores = p.part + up((int64_t)kGrid * 2 * p.nt * 8 * (c.dim + 4 + 2) * 4);
-    // every token of every page, and a started tile for each sequence
-    p.score_tiles = weigh ? ((int64_t)c.pages * c.page / kTile + c.batch) * c.kv_heads * p.subs : 0;
+    // every token of every page, and the places behind the groups' last tiles
+    p.score_tiles = weigh ? ((int64_t)c.pages * c.page / kTile + (int64_t)c.batch * kStart) * c.kv_heads * p.subs : 0;
     p.bytes = p.scores + up(p.score_tiles * kTile * p.nt * 8 * 4);
     return true;
 }
@@ -918,8 +930,17 @@ template <int KIND, int D, int NT>
 int launch(const AttendArgs& a, cudaStream_t stream) {
     using A = Attend<KIND, D, NT>;
     auto kernel = attend_kernel<KIND, D, NT>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename A::Smem));
+    // once per device (a repetition by another thread does no harm)
+    static std::atomic<uint64_t> told{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
+    const uint64_t bit = (uint64_t)1 << (device & 63);
+    if ((told.load(std::memory_order_relaxed) & bit) == 0) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename A::Smem));
+        if (e != cudaSuccess) return (int)e;
+        told.fetch_or(bit, std::memory_order_relaxed);
+    }
     kernel<<<kGrid, A::kWarps * 32, sizeof(typename A::Smem), stream>>>(a);
     return (int)cudaGetLastError();
 }

@@ -146,8 +146,10 @@ class KVCache:
                               ptr(seen), ptr(self.status), None, 0, *strides, pages, page, heads, dim, batch, table.shape[1],
                               KINDS[self.kind], 0)
         self._p = ctypes.addressof(self._c)
+        self._index = self.device.index
+        self._current_device, self._raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
         self._workspaces = []               # replaced ones stay: kernels in flight may use them
-        self._sizes = {}
+        self._sizes = {}                    # what a call's shapes have been found to be good for
         self._room(self.lib.rans_kv_counter_bytes(self._p))
 
     def _room(self, nbytes):
@@ -160,27 +162,35 @@ class KVCache:
             self._c.workspace, self._c.workspace_bytes = ws.data_ptr(), nbytes
 
     def _stream(self):
-        torch = self._torch
-        if torch.cuda.current_device() != self.device.index:
+        if self._current_device() != self._index:
             raise ValueError(f"the cache is on {self.device}; make it the current device")
-        return torch.cuda.current_stream().cuda_stream
+        return self._raw_stream(self._index)
 
-    def _rows(self, x, what):
+    def _rows(self, k, v):
+        """Checks of append's rows, which depend on their shapes alone: (type, bytes a value, strides are usable)."""
         torch = self._torch
-        _need(x.device == self.device and x.dim() == 3 and tuple(x.shape[1:]) == (self.kv_heads, self.dim),
-              f"{what} must be [tokens, {self.kv_heads}, {self.dim}] on {self.device}")
-        size = x.element_size()
-        if x.stride(2) != 1 or x.stride(0) * size % 16 or x.stride(1) * size % 16 or x.data_ptr() % 16:
-            x = x.contiguous().clone() if x.is_contiguous() else x.contiguous()
-        given = {torch.bfloat16: 0, torch.float16: 1, torch.float32: _FP32}.get(x.dtype)
-        _need(given is not None, f"{what} must be bf16, fp16 or fp32")
-        return x, given, size
+        for x, what in ((k, "k"), (v, "v")):
+            _need(x.device == self.device and x.dim() == 3 and tuple(x.shape[1:]) == (self.kv_heads, self.dim),
+                  f"{what} must be [tokens, {self.kv_heads}, {self.dim}] on {self.device}")
+        _need(k.dtype == v.dtype and k.shape == v.shape, "k and v must be alike")
+        given = {torch.bfloat16: 0, torch.float16: 1, torch.float32: _FP32}.get(k.dtype)
+        _need(given is not None, "k and v must be bf16, fp16 or fp32")
+        size = k.element_size()
+        usable = lambda x: x.stride(2) == 1 and x.stride(0) * size % 16 == 0 and x.stride(1) * size % 16 == 0   # noqa: E731
+        return given, size, usable(k), usable(v)
+
+    @staticmethod
+    def _aligned(x, usable):
+        """x itself, or a copy whose rows can be read 16 bytes at a time."""
+        if usable and x.data_ptr() % 16 == 0:
+            return x
+        return x.clone() if x.is_contiguous() else x.contiguous()
 
     def _starts(self, starts, tokens):
         if starts is None:
             _need(tokens == self.batch, f"without starts there is one token for each of the {self.batch} sequences")
             return None
-        _need(starts.dtype == self._torch.int32 and starts.device == self.device and starts.numel() == self.batch + 1
+        _need(starts.dtype == self._torch.int32 and starts.get_device() == self._index and starts.numel() == self.batch + 1
               and starts.is_contiguous(), f"starts must be contiguous int32 [{self.batch + 1}] on {self.device}")
         return starts.data_ptr()
 
@@ -225,12 +235,17 @@ class KVCache:
         """Append rows k, v [tokens, kv_heads, dim] (bf16, fp16 or fp32): row b to sequence b, or with starts (int32
         [batch + 1] on the device, rising from 0 to tokens) rows starts[b]..starts[b+1]-1.  Their pages have to be
         reserved."""
-        k, given, size = self._rows(k, "k")
-        v, other, _ = self._rows(v, "v")
-        _need(given == other and v.shape == k.shape, "k and v must be alike")
-        n = k.shape[0]
-        rc = self.lib.rans_kv_append(self._p, k.data_ptr(), v.data_ptr(), given, k.stride(0) * size, k.stride(1) * size,
-                                     v.stride(0) * size, v.stride(1) * size, self._starts(starts, n), n, self._stream())
+        key = (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype)
+        known = self._sizes.get(key)
+        if known is None:
+            known = self._sizes[key] = self._rows(k, v)
+        given, size, k_usable, v_usable = known
+        _need(k.get_device() == self._index and v.get_device() == self._index, f"k and v must be on {self.device}")
+        k, v, n = self._aligned(k, k_usable), self._aligned(v, v_usable), k.shape[0]
+        kt, kh, _ = k.stride()
+        vt, vh, _ = v.stride()
+        rc = self.lib.rans_kv_append(self._p, k.data_ptr(), v.data_ptr(), given, kt * size, kh * size, vt * size, vh * size,
+                                     self._starts(starts, n), n, self._stream())
         rb._check(rc, "rans_kv_append")
 
     def read(self, starts=None, tokens=None):
@@ -252,6 +267,33 @@ class KVCache:
         dim ** -0.5.  An empty sequence gives zeros and -inf.  weigh: also add each token's share of the attention,
         summed over a kv head's query heads, to `weight`."""
         torch = self._torch
+        key = (q.shape, q.stride(), q.dtype, weigh)
+        known = self._sizes.get(key)
+        if known is None:
+            known = self._sizes[key] = self._query(q, weigh)
+        kind, heads, usable = known
+        _need(q.get_device() == self._index, f"q must be on {self.device}")
+        q = self._aligned(q, usable)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        else:
+            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == self.device and out.is_contiguous()
+                  and out.data_ptr() % 16 == 0, "out must be contiguous and like q")
+        if log_sum is None:
+            log_sum = torch.empty((self.batch, heads), dtype=torch.float32, device=self.device)
+        else:
+            _need(log_sum.shape == (self.batch, heads) and log_sum.dtype == torch.float32 and log_sum.device == self.device
+                  and log_sum.is_contiguous(), "log_sum must be contiguous fp32 [batch, heads]")
+        q_batch, q_head, _ = q.stride()
+        rc = self.lib.rans_kv_attend(self._p, q.data_ptr(), kind, q_batch * 2, q_head * 2, heads,
+                                     self.dim ** -0.5 if scale is None else scale, out.data_ptr(), log_sum.data_ptr(),
+                                     1 if weigh else 0, self._stream())
+        rb._check(rc, "rans_kv_attend")
+        return out, log_sum
+
+    def _query(self, q, weigh):
+        """Checks of attend's query, which depend on its shape alone, and the workspace for it."""
+        torch = self._torch
         _need(q.dim() == 3 and q.shape[0] == self.batch and q.shape[2] == self.dim and q.device == self.device
               and q.shape[1] > 0 and q.shape[1] % self.kv_heads == 0,
               f"q must be [{self.batch}, a multiple of {self.kv_heads}, {self.dim}] on {self.device}")
@@ -259,29 +301,10 @@ class KVCache:
         _need(q.dtype in (torch.bfloat16, torch.float16) and (self.kind == "mxfp4" or kind == KINDS[self.kind]),
               f"q must be of the cache's type ({self.kind})")
         _need(not weigh or self.weight is not None, "this cache has no weight tensor")
-        if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-            q = q.contiguous().clone() if q.is_contiguous() else q.contiguous()
-        heads = q.shape[1]
-        key = (heads, weigh)
-        size = self._sizes.get(key)
-        if size is None:
-            size = self._sizes[key] = self.lib.rans_kv_attend_bytes(self._p, heads, int(weigh))
-            self._room(size)
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == self.device and out.is_contiguous()
-                  and out.data_ptr() % 16 == 0, "out must be contiguous and like q")
-        if log_sum is None:
-            log_sum = torch.empty(self.batch, heads, dtype=torch.float32, device=self.device)
-        else:
-            _need(log_sum.shape == (self.batch, heads) and log_sum.dtype == torch.float32 and log_sum.device == self.device
-                  and log_sum.is_contiguous(), "log_sum must be contiguous fp32 [batch, heads]")
-        rc = self.lib.rans_kv_attend(self._p, q.data_ptr(), kind, q.stride(0) * 2, q.stride(1) * 2, heads,
-                                     self.dim ** -0.5 if scale is None else scale, out.data_ptr(), log_sum.data_ptr(),
-                                     int(weigh), self._stream())
-        rb._check(rc, "rans_kv_attend")
-        return out, log_sum
+        size = self.lib.rans_kv_attend_bytes(self._p, q.shape[1], int(weigh))
+        _need(size > 0, f"{q.shape[1]} query heads on {self.kv_heads}, or the table's size, are more than the kernel counts")
+        self._room(size)
+        return kind, q.shape[1], q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0
 
     def evict(self, budget, recent=0):
         """Bring sequences with more than `budget` tokens back to it, per kv head: the `recent` newest tokens and the
