@@ -47,9 +47,10 @@ constexpr int kGrid = kSms;
 // A group's first tile waits for its page number and queries, and its end is written out: in the shares of work it
 // counts as this many tiles more (places without a tile behind the group's last one).
 constexpr int kStart = 2;
-// The maximum is only raised when a score passes it by this much (in powers of
-// two): probabilities then stay below 2^8, harmless in bf16, fp16 and fp32.
-constexpr float kSlack = 8.0f;
+// Probabilities are 2^(score - m) for a reference m that follows the running maximum from a distance: when a score passes
+// m + kHigh, m becomes the maximum - kRest.  Most tiles then leave O alone, the largest probability lies between 2^0 and
+// 2^15, and fp16 keeps probabilities down to 2^-36 of the largest instead of 2^-25.
+constexpr float kHigh = 15.0f, kRest = 11.0f;
 
 struct AttendArgs {
     RansKvCache c;
@@ -116,29 +117,30 @@ __device__ __forceinline__ uint32_t pack_as(int half, float lo, float hi) {
     return half ? pack2<true>(lo, hi) : pack2<false>(lo, hi);
 }
 
-// Two e2m1 codes (one byte) as fp16, exact.
-__device__ __forceinline__ uint32_t e2m1_to_half2(uint32_t byte) {
-    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// The e2m1 codes of a word's four bytes as four fp16 pairs (low half, high half of the byte), exact.
+__device__ __forceinline__ void e2m1_to_half(uint32_t (&r)[4], uint32_t w) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+}
+
+__device__ __forceinline__ uint32_t multiply2(uint32_t x, uint32_t f) {
+    const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&f));
+    return *reinterpret_cast<const uint32_t*>(&z);
 }
 
 // 2^e of a scale byte e + 127 (255: infinity, whose product with the zero codes of such a block is NaN).
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// The factors that turn two tokens' e2m1 codes, read as the low bits of bf16
-// (value * 2^-126), into value * 2^(e - 63): 2^(63 + e), a bf16 for every e the
-// format has.  The remaining 2^63 is applied to the output.
-__device__ __forceinline__ uint32_t factor2(uint32_t byte0, uint32_t byte1) {
-    return (min(byte0 + 63u, 255u) << 7) | (min(byte1 + 63u, 255u) << 23);
-}
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 __device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
 
 template <int KIND, int D, int NT>
 struct Attend {
     static constexpr bool kFp4 = KIND == RANS_KV_MXFP4;
-    // Operand types: 4-bit keys are exact in fp16 (their scale is applied to the sums); 4-bit values times their scale need bf16's range.
-    static constexpr bool kHalfV = KIND == RANS_KV_FP16;
     static constexpr int HP = NT * 8;                         // heads of a tile, padded
     static constexpr int kChunks = D / 32;                    // 32 values of a row
     // One block of an SM's whole register file: fewer parts to join than from several blocks.
@@ -298,6 +300,9 @@ struct Attend {
         float o[D / 16][NT][4];
         float m[NT][2], l[NT][2];
         float qs[kFp4 ? NT : 1][2];      // 4-bit: the powers of two taken out of the two heads' queries, times scale
+        // 4-bit: O of the lane's D / 64 words is held in units of 2^(unit - 127), a power near the words' scales, so that
+        // the values' operands fit fp16 (exactly: they have two significant bits).
+        int unit[kFp4 ? D / 64 : 1];
     };
 
     // The queries of a head group, in the order of load_k()'s values, to the warp's place in shared memory
@@ -345,6 +350,10 @@ struct Attend {
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) qs[(t * kChunks + j) * 32 + lane] = q[j];
             s.m[t][0] = s.m[t][1] = -INFINITY;
+            if constexpr (kFp4) {
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) s.unit[j] = 0;
+            }
             s.l[t][0] = s.l[t][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) s.o[i][t][0] = s.o[i][t][1] = s.o[i][t][2] = s.o[i][t][3] = 0.0f;
@@ -375,11 +384,8 @@ struct Attend {
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 uint32_t w0[4], w1[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w0[i] = e2m1_to_half2((r.w[0][j] >> (8 * i)) & 255);
-                    w1[i] = e2m1_to_half2((r.w[1][j] >> (8 * i)) & 255);
-                }
+                e2m1_to_half(w0, r.w[0][j]);
+                e2m1_to_half(w1, r.w[1][j]);
                 const float f0 = scale_of((r.s[0][j / 4] >> (8 * (j % 4))) & 255);
                 const float f1 = scale_of((r.s[1][j / 4] >> (8 * (j % 4))) & 255);
 #pragma unroll
@@ -402,9 +408,9 @@ struct Attend {
         }
     }
 
-    // The softmax's part of a tile of `valid` tokens: scores become P^T's operands, the maximum, the sum and O follow.
-    static __device__ __forceinline__ void probabilities(State& s, float (&sc)[NT][4], uint32_t (&pb)[NT][2], const AttendArgs& a,
-                                                         int64_t x, int valid, int lane) {
+    // The softmax's part of a tile of `valid` tokens: scores become probabilities, the maximum, the sum and O follow.
+    static __device__ __forceinline__ void probabilities(State& s, float (&sc)[NT][4], const AttendArgs& a, int64_t x, int valid,
+                                                         int lane) {
         const int g = lane >> 2, q4 = lane & 3;
         bool raise_max = false;
 #pragma unroll
@@ -418,7 +424,7 @@ struct Attend {
                 *reinterpret_cast<float2*>(p) = make_float2(sc[t][0], sc[t][1]);
                 *reinterpret_cast<float2*>(p + 8 * HP) = make_float2(sc[t][2], sc[t][3]);
             }
-            raise_max |= fmaxf(sc[t][0], sc[t][2]) > s.m[t][0] + kSlack || fmaxf(sc[t][1], sc[t][3]) > s.m[t][1] + kSlack;
+            raise_max |= fmaxf(sc[t][0], sc[t][2]) > s.m[t][0] + kHigh || fmaxf(sc[t][1], sc[t][3]) > s.m[t][1] + kHigh;
         }
         if (__any_sync(~0u, raise_max)) {
 #pragma unroll
@@ -429,7 +435,7 @@ struct Attend {
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-                    m = fmaxf(m, s.m[t][e]);
+                    m = fmaxf(m - kRest, s.m[t][e]);
                     const float f = m == -INFINITY ? 1.0f : exp2_fast(s.m[t][e] - m);
                     s.m[t][e] = m;
                     s.l[t][e] *= f;
@@ -443,20 +449,32 @@ struct Attend {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float m0 = s.m[t][0] == -INFINITY ? 0.0f : s.m[t][0], m1 = s.m[t][1] == -INFINITY ? 0.0f : s.m[t][1];
-            const float p0 = exp2_fast(sc[t][0] - m0), p1 = exp2_fast(sc[t][1] - m1);
-            const float p2 = exp2_fast(sc[t][2] - m0), p3 = exp2_fast(sc[t][3] - m1);
-            s.l[t][0] += p0 + p2;
-            s.l[t][1] += p1 + p3;
-            pb[t][0] = transpose8x8(pack2<kHalfV>(p0, p1));
-            pb[t][1] = transpose8x8(pack2<kHalfV>(p2, p3));
+            sc[t][0] = exp2_fast(sc[t][0] - m0);
+            sc[t][1] = exp2_fast(sc[t][1] - m1);
+            sc[t][2] = exp2_fast(sc[t][2] - m0);
+            sc[t][3] = exp2_fast(sc[t][3] - m1);
+            s.l[t][0] += sc[t][0] + sc[t][2];
+            s.l[t][1] += sc[t][1] + sc[t][3];
+        }
+    }
+
+    // P^T's operands from a tile's probabilities.
+    template <bool HALF>
+    static __device__ __forceinline__ void pack_probabilities(uint32_t (&pb)[NT][2], const float (&p)[NT][4]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            pb[t][0] = transpose8x8(pack2<HALF>(p[t][0], p[t][1]));
+            pb[t][1] = transpose8x8(pack2<HALF>(p[t][2], p[t][3]));
         }
     }
 
     // O^T += V^T P^T.
-    static __device__ __forceinline__ void accumulate(State& s, const RawV& r, const uint32_t (&pb)[NT][2]) {
+    static __device__ __forceinline__ void accumulate(State& s, const RawV& r, const float (&p)[NT][4]) {
+        uint32_t pb[NT][2];
+        if constexpr (!kFp4) {
+            pack_probabilities<KIND == RANS_KV_FP16>(pb, p);
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-            if constexpr (!kFp4) {
+            for (int j = 0; j < D / 64; ++j) {
                 const uint32_t* v0 = &r.v[0][j].x;
                 const uint32_t* v1 = &r.v[1][j].x;
                 const uint32_t* v2 = &r.v[2][j].x;
@@ -466,41 +484,123 @@ struct Attend {
                     const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
                     const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) mma<kHalfV>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                    for (int t = 0; t < NT; ++t) mma<KIND == RANS_KV_FP16>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                }
+            }
+        } else {
+            // fp16 factors 2^(scale byte - unit), for bytes from unit - 7 to unit + 8
+            uint32_t f[D / 64][2];
+            auto factors = [&]() {
+                uint32_t outside = 0;
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) {
+                    const uint32_t low = (uint32_t)(s.unit[j] - 7) * 0x10001u;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        // the two tokens' scale bytes, one in each half (byte 3 is zero where a lane loads fewer than four)
+                        const uint32_t u = D == 256 ? __byte_perm(r.s[2 * k], r.s[2 * k + 1], j | (j << 4) | ((4 + j) << 8) | ((4 + j) << 12)) & 0x00ff00ffu
+                                                    : __byte_perm(r.s[2 * k], r.s[2 * k + 1], j | (3 << 4) | ((4 + j) << 8) | (7 << 12));
+                        const uint32_t in = u - low;
+                        outside |= in;
+                        f[j][k] = in * 1024u + 0x20002000u;
+                    }
+                }
+                return __any_sync(~0u, (outside & 0xfff0fff0u) != 0);
+            };
+            bool wide = factors();
+            if (wide) {
+                raise_unit(s, r);
+                wide = factors();
+            }
+            if (!wide) {
+                pack_probabilities<true>(pb, p);
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) {
+                    // two tokens' codes of one column next to each other: columns 0, 2, 4, 6 and 1, 3, 5, 7
+                    const uint32_t even0 = (r.w[0][j] & 0x0f0f0f0fu) | ((r.w[1][j] << 4) & 0xf0f0f0f0u);
+                    const uint32_t odd0 = ((r.w[0][j] >> 4) & 0x0f0f0f0fu) | (r.w[1][j] & 0xf0f0f0f0u);
+                    const uint32_t even1 = (r.w[2][j] & 0x0f0f0f0fu) | ((r.w[3][j] << 4) & 0xf0f0f0f0u);
+                    const uint32_t odd1 = ((r.w[2][j] >> 4) & 0x0f0f0f0fu) | (r.w[3][j] & 0xf0f0f0f0u);
+                    uint32_t e0[4], o0[4], e1[4], o1[4];
+                    e2m1_to_half(e0, even0);
+                    e2m1_to_half(o0, odd0);
+                    e2m1_to_half(e1, even1);
+                    e2m1_to_half(o1, odd1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a0 = multiply2(e0[i], f[j][0]), a1 = multiply2(o0[i], f[j][0]);
+                        const uint32_t a2 = multiply2(e1[i], f[j][1]), a3 = multiply2(o1[i], f[j][1]);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) mma<true>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                    }
                 }
             } else {
-                const uint32_t lo01 = __byte_perm(r.w[0][j], r.w[1][j], 0x5410), hi01 = __byte_perm(r.w[0][j], r.w[1][j], 0x7632);
-                const uint32_t lo23 = __byte_perm(r.w[2][j], r.w[3][j], 0x5410), hi23 = __byte_perm(r.w[2][j], r.w[3][j], 0x7632);
-                const uint32_t f01 = factor2((r.s[0] >> (8 * j)) & 255, (r.s[1] >> (8 * j)) & 255);
-                const uint32_t f23 = factor2((r.s[2] >> (8 * j)) & 255, (r.s[3] >> (8 * j)) & 255);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    auto value = [&](uint32_t w, uint32_t f) {
-                        const uint32_t y = w << (12 - 4 * i);         // the code in the top bits of each half
-                        const uint32_t bits = (y & 0x80008000u) | ((y >> 6) & 0x01C001C0u);
-                        const __nv_bfloat162 z = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), *reinterpret_cast<const __nv_bfloat162*>(&f));
-                        return *reinterpret_cast<const uint32_t*>(&z);
-                    };
-                    const uint32_t a0 = value(lo01, f01), a1 = value(hi01, f01), a2 = value(lo23, f23), a3 = value(hi23, f23);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) mma<kHalfV>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
-                }
+                accumulate_wide(s, r, p);
             }
         }
     }
 
-    // First of the 8 consecutive values that o[j * 4 .. j * 4 + 3] of lane group g hold, and which
-    // accumulator holds value e: 16-bit rows pair neighbours, 4-bit rows pair e and e + 4.
+    // 4-bit: a new unit for words whose scales are above what the present one takes, from their largest scale.
+    static __device__ __forceinline__ void raise_unit(State& s, const RawV& r) {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            int top = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int byte = (int)((r.s[i] >> (8 * j)) & 255);
+                top = byte == 255 ? top : max(top, byte);
+            }
+            top = max(top, __shfl_xor_sync(~0u, top, 1));        // over the tile's tokens, of one lane group's words
+            top = max(top, __shfl_xor_sync(~0u, top, 2));
+            if (top <= (s.unit[j] == 0 ? 0 : s.unit[j] + 8)) continue;
+            const float down = s.unit[j] - top < -126 ? 0.0f : power_of_two(s.unit[j] - top);
+            s.unit[j] = top;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s.o[j * 4 + i][t][e] *= down;
+        }
+    }
+
+    // 4-bit: a tile whose scales are too far apart for fp16 (or that has a block of NaN): bf16 operands, any scale.
+    static __device__ __forceinline__ void accumulate_wide(State& s, const RawV& r, const float (&p)[NT][4]) {
+        uint32_t pb[NT][2];
+        pack_probabilities<false>(pb, p);
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int byte = (int)((r.s[i] >> (8 * j)) & 255);
+                f[i] = byte == 255 ? __uint_as_float(0x7fc00000u) : power_of_two(max(byte - s.unit[j], -126));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                auto value = [&](int token, int d) {
+                    const uint32_t code = (r.w[token][j] >> (4 * d)) & 15, n = code & 7;
+                    // 2^(n / 2 - 1) (1 + n % 2 / 2), or 0 and 0.5
+                    const float v = n < 2 ? 0.5f * (float)n : power_of_two((int)(n >> 1) - 1) * (n & 1 ? 1.5f : 1.0f);
+                    return (code & 8 ? -v : v) * f[token];
+                };
+                const uint32_t a0 = pack2<false>(value(0, 2 * i), value(1, 2 * i)), a1 = pack2<false>(value(0, 2 * i + 1), value(1, 2 * i + 1));
+                const uint32_t a2 = pack2<false>(value(2, 2 * i), value(3, 2 * i)), a3 = pack2<false>(value(2, 2 * i + 1), value(3, 2 * i + 1));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma<false>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+            }
+        }
+    }
+
+    // First of the 8 consecutive values that o[j * 4 .. j * 4 + 3] of lane group g hold, two each.
     static __device__ __forceinline__ int first_d(int j, int g) {
         if constexpr (!kFp4) return j * 64 + g * 8;
         const int w = g * (D / 64) + j;
         return (w % kChunks) * 32 + (w / kChunks) * 8;
     }
     static __device__ __forceinline__ float value_of(const State& s, int j, int t, int head, int e) {
-        return kFp4 ? s.o[j * 4 + (e & 3)][t][head + 2 * (e >> 2)] : s.o[j * 4 + (e >> 1)][t][head + 2 * (e & 1)];
+        return s.o[j * 4 + (e >> 1)][t][head + 2 * (e & 1)];
     }
-    // What the output still has to be multiplied by.
-    static __device__ __forceinline__ float out_scale() { return kFp4 ? 9.223372036854775808e18f : 1.0f; }
 
     static __device__ __forceinline__ void finish_head(const AttendArgs& a, int b, int head, float m, float l) {
         const int64_t i = (int64_t)b * a.heads + head;
@@ -508,8 +608,21 @@ struct Attend {
         if (a.weigh) a.stats[i] = make_float2(m == -INFINITY ? 0.0f : m, l > 0.0f || l != l ? 1.0f / l : 0.0f);
     }
 
-    // A warp's state: into `part` (smem) or, when it is the whole of a (sequence, head group), to the output.
-    static __device__ __forceinline__ void reduce_sum(State& s) {
+    // A warp's state once its tiles are done: sums over the lanes, O in units of one.  It goes into a part, or to the output
+    // when it is the whole of a group.
+    static __device__ __forceinline__ void finish(State& s) {
+        if constexpr (kFp4) {
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+                const float up = s.unit[j] == 0 ? 1.0f : power_of_two(s.unit[j] - 127);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s.o[j * 4 + i][t][e] *= up;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -528,7 +641,7 @@ struct Attend {
             for (int e = 0; e < 2; ++e) {
                 const int head = t * 8 + 2 * q4 + e;
                 if (head >= heads) continue;
-                const float l = s.l[t][e], f = l > 0.0f || l != l ? out_scale() / l : 0.0f;
+                const float l = s.l[t][e], f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
                 char* o = static_cast<char*>(a.out) + ((int64_t)b * a.heads + head0 + head) * D * 2;
 #pragma unroll
                 for (int j = 0; j < D / 64; ++j) {
@@ -602,7 +715,7 @@ struct Attend {
     }
 
     static __device__ __forceinline__ void store_joined(const AttendArgs& a, int b, int head, int d, float4 o, float m, float l) {
-        const float f = l > 0.0f || l != l ? out_scale() / l : 0.0f;
+        const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         uint2 w;
         w.x = pack_as(a.q_half, o.x * f, o.y * f);
         w.y = pack_as(a.q_half, o.z * f, o.w * f);
@@ -730,7 +843,6 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         // next scores are: the same registers, refilled as soon as their contents are used.
         while (true) {
             float sc[NT][4];
-            uint32_t pb[NT][2];
             bool more = true, ends = false;
             const Group now = s;
             if (have) {
@@ -747,11 +859,11 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                 A::load_k(rk, c, u, lane);
             }
             if (have) {
-                A::probabilities(st, sc, pb, a, x, valid, lane);
-                A::accumulate(st, rv, pb);
+                A::probabilities(st, sc, a, x, valid, lane);
+                A::accumulate(st, rv, sc);
                 x = next;
                 if (ends || !more) {
-                    A::reduce_sum(st);
+                    A::finish(st);
                     __syncwarp();
                     if (whole && ends) {
                         A::write_out(st, a, now.b, head0_of(now), heads_of(now), lane);
