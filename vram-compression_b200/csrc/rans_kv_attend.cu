@@ -77,6 +77,15 @@ __device__ __forceinline__ uint4 load16(const void* p) {
     return r;
 }
 
+// 16 bytes into shared memory, the first `size` of them from global memory, the rest zero.
+__device__ __forceinline__ void copy16(void* to, const void* from, int size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 :: "r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
 template <bool HALF>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -149,35 +158,58 @@ struct Attend {
 
     // What is left of a run of tiles of one group: O, and the running maximum and sum of each head; a warp's in shared
     // memory, a block's in the workspace.
-    struct Part {
+    struct alignas(16) Part {
         float o[HP][kRow];
         float2 ml[HP];
     };
 
+    // 4-bit tiles as they lie in the pages, copied a few tiles ahead.
+    static constexpr int kStages = 3;
+    struct alignas(16) Stage {
+        uint8_t k[kTile * D / 2], v[kTile * D / 2], ks[kTile * kChunks], vs[kTile * kChunks];
+    };
+    // A warp's second part is written when its last tile is done, in the place of its stages.
+    union Late {
+        Part part;
+        Stage stage[kFp4 ? kStages : 1];
+    };
+
     struct Smem {
-        Part part[kWarps * 2];               // the warps' parts: first parts, then second ones
+        Part part[kWarps];                   // the warps' first parts
+        Late late[kWarps];                   // their second ones
+        uint4 q[kWarps][NT * kChunks * 32];  // the queries that they work on
         int tag[kWarps * 2];                 // the group of each part
         int first_block[2], last_block[2], last[2];      // of the block's first and last group, if it has only some of it
         int warp_sum[kWarps];
         int pre[RANS_KV_MAX_BATCH + 1];      // places of one head in front of each sequence
     };
 
-    // One tile's rows as they come from memory.
+    // The token of a tile that row g (and, 8 further, row g + 8) of S^T stands for, and the one that a lane's i-th value row
+    // is (rows 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of P^T).  4-bit rows are read from shared memory, where neighbours in either
+    // order have to lie in different halves of the banks.
+    static __device__ __forceinline__ int key_row(int g) { return kFp4 ? (g & 6) | (((g >> 1) + g) & 1) : g; }
+    static __device__ __forceinline__ int value_row(int q4, int i) { return key_row(2 * q4 + (i & 1)) + 8 * (i >> 1); }
+
+    // One tile's rows in registers, 16 bits a value ..
     struct RawK {
-        uint4 k[kFp4 ? 1 : 2][kFp4 ? 1 : kChunks];            // rows g, g + 8
-        uint32_t w[kFp4 ? 2 : 1][kFp4 ? kChunks : 1];         // codes: word n = block n
-        uint32_t s[kFp4 ? 2 : 1][kFp4 ? (D + 127) / 128 : 1]; // scale bytes
+        uint4 k[2][kChunks];                                  // rows g, g + 8
     };
     struct RawV {
-        uint4 v[kFp4 ? 1 : 4][kFp4 ? 1 : D / 64];             // rows 2 q, 2 q + 1, 2 q + 8, 2 q + 9
-        uint32_t w[kFp4 ? 4 : 1][kFp4 ? D / 64 : 1];
-        uint32_t s[kFp4 ? 4 : 1];
+        uint4 v[4][D / 64];
+    };
+    // .. or 4: words of 8 codes, and scale bytes
+    struct CodeK {
+        uint32_t w[2][kChunks], s[2][(D + 127) / 128];        // word n = block n
+    };
+    struct CodeV {
+        uint32_t w[4][D / 64], s[4];
     };
 
-    // A lane's place in the tiles of one (sequence, kv head): pointers to its first key and value row of the current
-    // tile.  Within a page they step by 16 rows; the number of the following page is fetched a page ahead.
+    // A lane's place in the tiles of one (sequence, kv head).  Within a page it steps by 16 rows; the number of the following
+    // page is fetched a page ahead.
     struct Cursor {
-        const char *k, *v, *ks, *vs;
+        const char *k, *v;                       // 16 bits: the lane's first key and value row of the tile
+        int64_t row;                             // 4 bits: the tile's first row
         int slot, ahead, next, left, valid;      // left: tokens from the tile's first one on; valid: of them in the tile
 
         __device__ __forceinline__ void at_page(const RansKvCache& c, int h, int p, int lane) {
@@ -186,15 +218,11 @@ struct Attend {
             if (!ok) raise(c, RANS_KV_BAD_PAGE);
             valid = ok ? min(left, kTile) : 0;
             const int64_t pg = ok ? p : 0;
-            if constexpr (!kFp4) {
+            if constexpr (kFp4) {
+                row = (pg * c.kv_heads + h) * c.page + slot;
+            } else {
                 k = static_cast<const char*>(c.k) + pg * c.k_page + h * c.k_head + (slot + g) * c.k_slot + q4 * 16;
                 v = static_cast<const char*>(c.v) + pg * c.v_page + h * c.v_head + (slot + 2 * q4) * c.v_slot + g * 16;
-            } else {
-                const int64_t row = (pg * c.kv_heads + h) * c.page + slot;
-                k = static_cast<const char*>(c.k) + (row + g) * (D / 2) + q4 * (D / 8);
-                v = static_cast<const char*>(c.v) + (row + 2 * q4) * (D / 2) + g * (D / 16);
-                ks = reinterpret_cast<const char*>(c.k_scale) + (row + g) * kChunks;
-                vs = reinterpret_cast<const char*>(c.v_scale) + (row + 2 * q4) * kChunks + (g & 1) * (D / 64);
             }
         }
         __device__ __forceinline__ void fetch_next(const RansKvCache& c, int b) {
@@ -220,80 +248,104 @@ struct Attend {
                 return;
             }
             if (valid > 0) valid = min(left, kTile);
-            if constexpr (!kFp4) {
+            if constexpr (kFp4) {
+                row += kTile;
+            } else {
                 k += kTile * c.k_slot;
                 v += kTile * c.v_slot;
-            } else {
-                k += kTile * (D / 2);
-                v += kTile * (D / 2);
-                ks += kTile * kChunks;
-                vs += kTile * kChunks;
             }
         }
     };
 
     template <bool FULL>
-    static __device__ __forceinline__ void load_k(RawK& r, const RansKvCache& c, const Cursor& u, int lane) {
+    static __device__ __forceinline__ void load_k(RawK& r, const RansKvCache& c, const char* k, int valid, int lane) {
         const int g = lane >> 2;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const bool in = FULL || g + 8 * i < u.valid;
-            if constexpr (!kFp4) {
-                const char* p = u.k + 8 * i * c.k_slot;
+            const bool in = FULL || g + 8 * i < valid;
+            const char* p = k + 8 * i * c.k_slot;
 #pragma unroll
-                for (int j = 0; j < kChunks; ++j) r.k[i][j] = in ? load16(p + j * 64) : zero;
-            } else if constexpr (D == 64) {
-                const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(u.k + i * 8 * (D / 2))) : make_uint2(0, 0);
-                r.w[i][0] = w.x; r.w[i][1] = w.y;
-                r.s[i][0] = in ? __ldg(reinterpret_cast<const uint16_t*>(u.ks + i * 8 * kChunks)) : 0;
-            } else {
-#pragma unroll
-                for (int j = 0; j < kChunks; j += 4) {
-                    const uint4 w = in ? load16(u.k + i * 8 * (D / 2) + j * 4) : zero;
-                    r.w[i][j] = w.x; r.w[i][j + 1] = w.y; r.w[i][j + 2] = w.z; r.w[i][j + 3] = w.w;
-                    r.s[i][j / 4] = in ? __ldg(reinterpret_cast<const uint32_t*>(u.ks + i * 8 * kChunks + j)) : 0;
-                }
-            }
+            for (int j = 0; j < kChunks; ++j) r.k[i][j] = in ? load16(p + j * 64) : make_uint4(0, 0, 0, 0);
         }
     }
-
     template <bool FULL>
-    static __device__ __forceinline__ void load_v(RawV& r, const RansKvCache& c, const char* v, const char* vs, int valid, int lane) {
+    static __device__ __forceinline__ void load_v(RawV& r, const RansKvCache& c, const char* v, int valid, int lane) {
         const int q4 = lane & 3;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = (i & 1) + 8 * (i >> 1);
             const bool in = FULL || 2 * q4 + row < valid;
-            if constexpr (!kFp4) {
-                const char* p = v + row * c.v_slot;
+            const char* p = v + row * c.v_slot;
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) r.v[i][j] = in ? load16(p + j * 128) : zero;
+            for (int j = 0; j < D / 64; ++j) r.v[i][j] = in ? load16(p + j * 128) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    static __device__ __forceinline__ void load_k(RawK& r, const RansKvCache& c, const Cursor& u, int lane) {
+        if (u.valid == kTile) load_k<true>(r, c, u.k, u.valid, lane); else load_k<false>(r, c, u.k, u.valid, lane);
+    }
+    static __device__ __forceinline__ void load_v(RawV& r, const RansKvCache& c, const Cursor& u, int lane) {
+        if (u.valid == kTile) load_v<true>(r, c, u.v, u.valid, lane); else load_v<false>(r, c, u.v, u.valid, lane);
+    }
+
+    // Starts a 4-bit tile's copy into shared memory, 16 bytes a lane; what lies behind its last token becomes zero.
+    static __device__ __forceinline__ void copy_tile(Stage& st, const RansKvCache& c, const Cursor& u, int lane) {
+        const int at = lane * 16;
+        const uint8_t* k = static_cast<const uint8_t*>(c.k) + u.row * (D / 2) + at;
+        const uint8_t* v = static_cast<const uint8_t*>(c.v) + u.row * (D / 2) + at;
+#pragma unroll
+        for (int i = 0; i < kTile * D / 2; i += 512) {
+            const int size = min(max(u.valid * (D / 2) - at - i, 0), 16);
+            copy16(st.k + at + i, k + i, size);
+            copy16(st.v + at + i, v + i, size);
+        }
+        constexpr int kScaleLanes = kTile * kChunks / 16;
+        if (lane < 2 * kScaleLanes) {
+            const bool is_k = lane < kScaleLanes;
+            const int from = at - (is_k ? 0 : kTile * kChunks);
+            copy16(st.ks + at, (is_k ? c.k_scale : c.v_scale) + u.row * kChunks + from, min(max(u.valid * kChunks - from, 0), 16));
+        }
+    }
+
+    static __device__ __forceinline__ void read_k(CodeK& r, const Stage& st, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = key_row(g) + 8 * i;
+            const uint8_t* p = st.k + row * (D / 2) + q4 * (D / 8);
+            if constexpr (D == 64) {
+                const uint2 w = *reinterpret_cast<const uint2*>(p);
+                r.w[i][0] = w.x; r.w[i][1] = w.y;
+                r.s[i][0] = *reinterpret_cast<const uint16_t*>(st.ks + row * kChunks);
             } else {
-                const char* p = v + row * (D / 2);
-                const char* ps = vs + row * kChunks;
-                if constexpr (D == 256) {
-                    const uint4 w = in ? load16(p) : zero;
-                    r.w[i][0] = w.x; r.w[i][1] = w.y; r.w[i][2] = w.z; r.w[i][3] = w.w;
-                    r.s[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(ps)) : 0;
-                } else if constexpr (D == 128) {
-                    const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
-                    r.w[i][0] = w.x; r.w[i][1] = w.y;
-                    r.s[i] = in ? __ldg(reinterpret_cast<const uint16_t*>(ps)) : 0;
-                } else {
-                    r.w[i][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0;
-                    r.s[i] = in ? __ldg(reinterpret_cast<const uint8_t*>(ps)) : 0;
+#pragma unroll
+                for (int j = 0; j < kChunks; j += 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(p + j * 4);
+                    r.w[i][j] = w.x; r.w[i][j + 1] = w.y; r.w[i][j + 2] = w.z; r.w[i][j + 3] = w.w;
+                    r.s[i][j / 4] = *reinterpret_cast<const uint32_t*>(st.ks + row * kChunks + j);
                 }
             }
         }
     }
-
-    static __device__ __forceinline__ void load_k(RawK& r, const RansKvCache& c, const Cursor& u, int lane) {
-        if (u.valid == kTile) load_k<true>(r, c, u, lane); else load_k<false>(r, c, u, lane);
-    }
-    static __device__ __forceinline__ void load_v(RawV& r, const RansKvCache& c, const char* v, const char* vs, int valid, int lane) {
-        if (valid == kTile) load_v<true>(r, c, v, vs, valid, lane); else load_v<false>(r, c, v, vs, valid, lane);
+    static __device__ __forceinline__ void read_v(CodeV& r, const Stage& st, int lane) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = value_row(q4, i);
+            const uint8_t* p = st.v + row * (D / 2) + g * (D / 16);
+            const uint8_t* s = st.vs + row * kChunks + (g & 1) * (D / 64);
+            if constexpr (D == 256) {
+                const uint4 w = *reinterpret_cast<const uint4*>(p);
+                r.w[i][0] = w.x; r.w[i][1] = w.y; r.w[i][2] = w.z; r.w[i][3] = w.w;
+                r.s[i] = *reinterpret_cast<const uint32_t*>(s);
+            } else if constexpr (D == 128) {
+                const uint2 w = *reinterpret_cast<const uint2*>(p);
+                r.w[i][0] = w.x; r.w[i][1] = w.y;
+                r.s[i] = *reinterpret_cast<const uint16_t*>(s);
+            } else {
+                r.w[i][0] = *reinterpret_cast<const uint32_t*>(p);
+                r.s[i] = *s;
+            }
+        }
     }
 
     struct State {
@@ -362,65 +414,68 @@ struct Attend {
     }
 
     // S^T of a tile, scaled to powers of two.
-    static __device__ __forceinline__ void scores(const State& s, const uint4* qs, const RawK& r, const AttendArgs& a, float (&sc)[NT][4], int lane) {
+    static __device__ __forceinline__ void scores(const State& s, const uint4* qs, const RawK& r, const AttendArgs& a,
+                                                  float (&sc)[NT][4], int lane) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
-        if constexpr (!kFp4) {
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                const uint4 k0 = r.k[0][j], k1 = r.k[1][j];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint4 q = qs[(t * kChunks + j) * 32 + lane];
-                    mma<KIND == RANS_KV_FP16>(sc[t], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
-                    mma<KIND == RANS_KV_FP16>(sc[t], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[t][i] *= a.scale_log2;
-        } else {
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                uint32_t w0[4], w1[4];
-                e2m1_to_half(w0, r.w[0][j]);
-                e2m1_to_half(w1, r.w[1][j]);
-                const float f0 = scale_of((r.s[0][j / 4] >> (8 * (j % 4))) & 255);
-                const float f1 = scale_of((r.s[1][j / 4] >> (8 * (j % 4))) & 255);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const uint4 q = qs[(t * kChunks + j) * 32 + lane];
-                    mma<true>(d, w0[0], w1[0], w0[1], w1[1], q.x, q.y);
-                    mma<true>(d, w0[2], w1[2], w0[3], w1[3], q.z, q.w);
-                    sc[t][0] = fmaf(d[0], f0, sc[t][0]);
-                    sc[t][1] = fmaf(d[1], f0, sc[t][1]);
-                    sc[t][2] = fmaf(d[2], f1, sc[t][2]);
-                    sc[t][3] = fmaf(d[3], f1, sc[t][3]);
-                }
-            }
+        for (int j = 0; j < kChunks; ++j) {
+            const uint4 k0 = r.k[0][j], k1 = r.k[1][j];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                sc[t][0] *= s.qs[t][0]; sc[t][1] *= s.qs[t][1];
-                sc[t][2] *= s.qs[t][0]; sc[t][3] *= s.qs[t][1];
+                const uint4 q = qs[(t * kChunks + j) * 32 + lane];
+                mma<KIND == RANS_KV_FP16>(sc[t], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
+                mma<KIND == RANS_KV_FP16>(sc[t], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
             }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][i] *= a.scale_log2;
+    }
+    static __device__ __forceinline__ void scores(const State& s, const uint4* qs, const CodeK& r, const AttendArgs& a,
+                                                  float (&sc)[NT][4], int lane) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            uint32_t w0[4], w1[4];
+            e2m1_to_half(w0, r.w[0][j]);
+            e2m1_to_half(w1, r.w[1][j]);
+            const float f0 = scale_of((r.s[0][j / 4] >> (8 * (j % 4))) & 255);
+            const float f1 = scale_of((r.s[1][j / 4] >> (8 * (j % 4))) & 255);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint4 q = qs[(t * kChunks + j) * 32 + lane];
+                mma<true>(d, w0[0], w1[0], w0[1], w1[1], q.x, q.y);
+                mma<true>(d, w0[2], w1[2], w0[3], w1[3], q.z, q.w);
+                sc[t][0] = fmaf(d[0], f0, sc[t][0]);
+                sc[t][1] = fmaf(d[1], f0, sc[t][1]);
+                sc[t][2] = fmaf(d[2], f1, sc[t][2]);
+                sc[t][3] = fmaf(d[3], f1, sc[t][3]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            sc[t][0] *= s.qs[t][0]; sc[t][1] *= s.qs[t][1];
+            sc[t][2] *= s.qs[t][0]; sc[t][3] *= s.qs[t][1];
         }
     }
 
-    // The softmax's part of a tile of `valid` tokens: scores become probabilities, the maximum, the sum and O follow.
+    // The softmax's part of a tile with `valid` tokens: scores become probabilities, the maximum, the sum and O follow.
     static __device__ __forceinline__ void probabilities(State& s, float (&sc)[NT][4], const AttendArgs& a, int64_t x, int valid,
                                                          int lane) {
-        const int g = lane >> 2, q4 = lane & 3;
+        const int q4 = lane & 3, row = key_row(lane >> 2);
         bool raise_max = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if (valid < kTile) {
-                if (g >= valid) sc[t][0] = sc[t][1] = -INFINITY;
-                if (g + 8 >= valid) sc[t][2] = sc[t][3] = -INFINITY;
+                if (row >= valid) sc[t][0] = sc[t][1] = -INFINITY;
+                if (row + 8 >= valid) sc[t][2] = sc[t][3] = -INFINITY;
             }
             if (a.weigh && x < a.score_tiles) {
-                float* p = a.scores + (x * kTile + g) * HP + t * 8 + 2 * q4;
+                float* p = a.scores + (x * kTile + row) * HP + t * 8 + 2 * q4;
                 *reinterpret_cast<float2*>(p) = make_float2(sc[t][0], sc[t][1]);
                 *reinterpret_cast<float2*>(p + 8 * HP) = make_float2(sc[t][2], sc[t][3]);
             }
@@ -471,77 +526,79 @@ struct Attend {
     // O^T += V^T P^T.
     static __device__ __forceinline__ void accumulate(State& s, const RawV& r, const float (&p)[NT][4]) {
         uint32_t pb[NT][2];
-        if constexpr (!kFp4) {
-            pack_probabilities<KIND == RANS_KV_FP16>(pb, p);
+        pack_probabilities<KIND == RANS_KV_FP16>(pb, p);
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-                const uint32_t* v0 = &r.v[0][j].x;
-                const uint32_t* v1 = &r.v[1][j].x;
-                const uint32_t* v2 = &r.v[2][j].x;
-                const uint32_t* v3 = &r.v[3][j].x;
+        for (int j = 0; j < D / 64; ++j) {
+            const uint32_t* v0 = &r.v[0][j].x;
+            const uint32_t* v1 = &r.v[1][j].x;
+            const uint32_t* v2 = &r.v[2][j].x;
+            const uint32_t* v3 = &r.v[3][j].x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
-                    const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
+                const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) mma<KIND == RANS_KV_FP16>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
-                }
+                for (int t = 0; t < NT; ++t) mma<KIND == RANS_KV_FP16>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
             }
-        } else {
-            // fp16 factors 2^(scale byte - unit), for bytes from unit - 7 to unit + 8
-            uint32_t f[D / 64][2];
-            auto factors = [&]() {
-                uint32_t outside = 0;
+        }
+    }
+
+    // fp16 factors 2^(scale byte - unit) of a lane's words, for bytes from unit - 7 to unit + 8; whether some tile's are outside.
+    static __device__ __forceinline__ bool factors(uint32_t (&f)[D / 64][2], const State& s, const CodeV& r) {
+        uint32_t outside = 0;
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-                    const uint32_t low = (uint32_t)(s.unit[j] - 7) * 0x10001u;
+        for (int j = 0; j < D / 64; ++j) {
+            const uint32_t low = (uint32_t)(s.unit[j] - 7) * 0x10001u;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        // the two tokens' scale bytes, one in each half (byte 3 is zero where a lane loads fewer than four)
-                        const uint32_t u = D == 256 ? __byte_perm(r.s[2 * k], r.s[2 * k + 1], j | (j << 4) | ((4 + j) << 8) | ((4 + j) << 12)) & 0x00ff00ffu
-                                                    : __byte_perm(r.s[2 * k], r.s[2 * k + 1], j | (3 << 4) | ((4 + j) << 8) | (7 << 12));
-                        const uint32_t in = u - low;
-                        outside |= in;
-                        f[j][k] = in * 1024u + 0x20002000u;
-                    }
-                }
-                return __any_sync(~0u, (outside & 0xfff0fff0u) != 0);
-            };
-            bool wide = factors();
-            if (wide) {
-                raise_unit(s, r);
-                wide = factors();
+            for (int k = 0; k < 2; ++k) {
+                // the two tokens' scale bytes, one in each half (byte 3 is zero where a lane has fewer than four)
+                const uint32_t u = D == 256 ? __byte_perm(r.s[2 * k], r.s[2 * k + 1], j | (j << 4) | ((4 + j) << 8) | ((4 + j) << 12)) & 0x00ff00ffu
+                                            : __byte_perm(r.s[2 * k], r.s[2 * k + 1], j | (3 << 4) | ((4 + j) << 8) | (7 << 12));
+                const uint32_t in = u - low;
+                outside |= in;
+                f[j][k] = in * 1024u + 0x20002000u;
             }
-            if (!wide) {
-                pack_probabilities<true>(pb, p);
+        }
+        return __any_sync(~0u, (outside & 0xfff0fff0u) != 0);
+    }
+
+    static __device__ __forceinline__ void accumulate(State& s, const CodeV& r, const float (&p)[NT][4]) {
+        uint32_t f[D / 64][2];
+        bool wide = factors(f, s, r);
+        if (wide) {
+            raise_unit(s, r);
+            wide = factors(f, s, r);
+        }
+        if (wide) {
+            accumulate_wide(s, r, p);
+            return;
+        }
+        uint32_t pb[NT][2];
+        pack_probabilities<true>(pb, p);
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-                    // two tokens' codes of one column next to each other: columns 0, 2, 4, 6 and 1, 3, 5, 7
-                    const uint32_t even0 = (r.w[0][j] & 0x0f0f0f0fu) | ((r.w[1][j] << 4) & 0xf0f0f0f0u);
-                    const uint32_t odd0 = ((r.w[0][j] >> 4) & 0x0f0f0f0fu) | (r.w[1][j] & 0xf0f0f0f0u);
-                    const uint32_t even1 = (r.w[2][j] & 0x0f0f0f0fu) | ((r.w[3][j] << 4) & 0xf0f0f0f0u);
-                    const uint32_t odd1 = ((r.w[2][j] >> 4) & 0x0f0f0f0fu) | (r.w[3][j] & 0xf0f0f0f0u);
-                    uint32_t e0[4], o0[4], e1[4], o1[4];
-                    e2m1_to_half(e0, even0);
-                    e2m1_to_half(o0, odd0);
-                    e2m1_to_half(e1, even1);
-                    e2m1_to_half(o1, odd1);
+        for (int j = 0; j < D / 64; ++j) {
+            // two tokens' codes of one column next to each other: columns 0, 2, 4, 6 and 1, 3, 5, 7
+            const uint32_t even0 = (r.w[0][j] & 0x0f0f0f0fu) | ((r.w[1][j] << 4) & 0xf0f0f0f0u);
+            const uint32_t odd0 = ((r.w[0][j] >> 4) & 0x0f0f0f0fu) | (r.w[1][j] & 0xf0f0f0f0u);
+            const uint32_t even1 = (r.w[2][j] & 0x0f0f0f0fu) | ((r.w[3][j] << 4) & 0xf0f0f0f0u);
+            const uint32_t odd1 = ((r.w[2][j] >> 4) & 0x0f0f0f0fu) | (r.w[3][j] & 0xf0f0f0f0u);
+            uint32_t e0[4], o0[4], e1[4], o1[4];
+            e2m1_to_half(e0, even0);
+            e2m1_to_half(o0, odd0);
+            e2m1_to_half(e1, even1);
+            e2m1_to_half(o1, odd1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t a0 = multiply2(e0[i], f[j][0]), a1 = multiply2(o0[i], f[j][0]);
-                        const uint32_t a2 = multiply2(e1[i], f[j][1]), a3 = multiply2(o1[i], f[j][1]);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a0 = multiply2(e0[i], f[j][0]), a1 = multiply2(o0[i], f[j][0]);
+                const uint32_t a2 = multiply2(e1[i], f[j][1]), a3 = multiply2(o1[i], f[j][1]);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) mma<true>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
-                    }
-                }
-            } else {
-                accumulate_wide(s, r, p);
+                for (int t = 0; t < NT; ++t) mma<true>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
             }
         }
     }
 
     // 4-bit: a new unit for words whose scales are above what the present one takes, from their largest scale.
-    static __device__ __forceinline__ void raise_unit(State& s, const RawV& r) {
+    static __device__ __forceinline__ void raise_unit(State& s, const CodeV& r) {
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             int top = 0;
@@ -565,7 +622,7 @@ struct Attend {
     }
 
     // 4-bit: a tile whose scales are too far apart for fp16 (or that has a block of NaN): bf16 operands, any scale.
-    static __device__ __forceinline__ void accumulate_wide(State& s, const RawV& r, const float (&p)[NT][4]) {
+    static __device__ __forceinline__ void accumulate_wide(State& s, const CodeV& r, const float (&p)[NT][4]) {
         uint32_t pb[NT][2];
         pack_probabilities<false>(pb, p);
 #pragma unroll
@@ -787,6 +844,8 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                 if (i < a.heads && a.log_sum != nullptr) a.log_sum[(int64_t)b * a.heads + i] = -INFINITY;
             }
 
+    static_assert(sizeof(typename A::Smem) <= 227 * 1024, "a block's shared memory");
+    static_assert(sizeof(typename A::Part) == sizeof(float) * HP * (D + 6), "make_plan's size of a part");
     static_assert(kThreads >= kGrid, "a thread for every block");
     // Equal runs of places: per block, and in it per warp.
     const int blocks = min((int)gridDim.x, (total + W - 1) / W);       // each of their warps has a tile
@@ -803,7 +862,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
 
     Group s{};
     int nt = 0, tile = 0;
-    auto next_group = [&]() {
+    auto next_group = [&](Group& s, int& nt, int& tile) {
         tile = 0;
         if (++s.sub < a.subs) return;
         s.sub = 0;
@@ -826,62 +885,114 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         s.sub = seg - s.h * a.subs;
         if (tile >= nt) {                               // behind a group's last tile
             x += nt + kStart - tile;
-            next_group();
+            next_group(s, nt, tile);
         }
     }
     if (x < xe) {
-        // A warp's second part is written when it is done, so until then its queries live there.
-        uint4* qs = reinterpret_cast<uint4*>(&sm.part[W + warp]);
-        static_assert(sizeof(typename A::Part) >= NT * A::kChunks * 32 * sizeof(uint4), "room for the queries");
+        uint4* qs = sm.q[warp];
         typename A::State st;
         typename A::Cursor u;
-        typename A::RawK rk;
-        typename A::RawV rv;
-        int flushed = 0, valid = 0, next = 0;
-        bool have = false, whole = false, fresh = true;
-        // Keys of the next tile are on their way while this tile's softmax and values are worked on, and values while the
-        // next scores are: the same registers, refilled as soon as their contents are used.
-        while (true) {
-            float sc[NT][4];
-            bool more = true, ends = false;
-            const Group now = s;
-            if (have) {
-                A::scores(st, qs, rk, a, sc, lane);
-                ends = ++tile == nt;
-                next = x + 1 + (ends ? kStart : 0);
-                more = next < xe;
-                valid = u.valid;
-                fresh = ends;
-                if (ends && more) next_group();
+        int flushed = 0;
+        bool whole = tile == 0;
+        auto flush = [&](const Group& of, bool ends) {
+            A::finish(st);
+            __syncwarp();
+            if (whole && ends) {
+                A::write_out(st, a, of.b, head0_of(of), heads_of(of), lane);
+            } else {
+                A::write_part(st, flushed == 0 ? sm.part[warp] : sm.late[warp].part, lane);
+                if (lane == 0) sm.tag[flushed * W + warp] = of.pack();
+                ++flushed;
             }
-            if (more) {
-                if (fresh) u.begin(c, s.b, s.h, checked_length(c, s.b), tile, lane); else u.advance(c, s.b, s.h, lane);
-                A::load_k(rk, c, u, lane);
-            }
-            if (have) {
-                A::probabilities(st, sc, a, x, valid, lane);
-                A::accumulate(st, rv, sc);
-                x = next;
-                if (ends || !more) {
-                    A::finish(st);
-                    __syncwarp();
-                    if (whole && ends) {
-                        A::write_out(st, a, now.b, head0_of(now), heads_of(now), lane);
-                    } else {
-                        A::write_part(st, sm.part[flushed * W + warp], lane);
-                        if (lane == 0) sm.tag[flushed * W + warp] = now.pack();
-                        ++flushed;
+        };
+        if constexpr (A::kFp4) {
+            // The copies run kStages - 1 tiles ahead, in places of their own (`ahead`).
+            constexpr int kStages = A::kStages;
+            typename A::Stage* stages = sm.late[warp].stage;
+            Group ahead = s;
+            int ahead_nt = nt, ahead_tile = tile, ahead_x = x;
+            uint32_t valid = 0;                          // of each stage, 8 bits
+            bool fresh = true, ahead_fresh = true;
+            auto copy = [&](int stage) {
+                if (ahead_x < xe) {
+                    if (ahead_fresh) u.begin(c, ahead.b, ahead.h, checked_length(c, ahead.b), ahead_tile, lane);
+                    else u.advance(c, ahead.b, ahead.h, lane);
+                    valid = (valid & ~(255u << (8 * stage))) | (uint32_t)u.valid << (8 * stage);
+                    A::copy_tile(stages[stage], c, u, lane);
+                    ++ahead_x;
+                    ahead_fresh = ++ahead_tile == ahead_nt;
+                    if (ahead_fresh) {
+                        ahead_x += kStart;
+                        if (ahead_x < xe) next_group(ahead, ahead_nt, ahead_tile);
                     }
                 }
+                copies_end();
+            };
+#pragma unroll 1
+            for (int i = 0; i < kStages - 1; ++i) copy(i);
+#pragma unroll 1
+            for (int stage = 0, free = kStages - 1;; free = stage, stage = stage == kStages - 1 ? 0 : stage + 1) {
+                if (fresh) A::begin(st, qs, a, s.b, head0_of(s), heads_of(s), lane);
+                copies_wait<kStages - 2>();
+                __syncwarp();                            // all lanes' copies of this tile are there, and the tile before it is read
+                copy(free);
+                float sc[NT][4];
+                typename A::CodeK ck;
+                A::read_k(ck, stages[stage], lane);
+                A::scores(st, qs, ck, a, sc, lane);
+                A::probabilities(st, sc, a, x, (int)(valid >> (8 * stage)) & 255, lane);
+                typename A::CodeV cv;
+                A::read_v(cv, stages[stage], lane);
+                A::accumulate(st, cv, sc);
+                fresh = ++tile == nt;
+                x += 1 + (fresh ? kStart : 0);
+                if (fresh || x >= xe) flush(s, fresh);
+                if (x >= xe) break;
+                if (fresh) {
+                    next_group(s, nt, tile);
+                    whole = true;
+                }
             }
-            if (!more) break;
-            if (fresh) {
-                whole = tile == 0;
-                A::begin(st, qs, a, s.b, head0_of(s), heads_of(s), lane);
-                fresh = false;
+        } else {
+            // Keys of the next tile are on their way while this tile's softmax and values are worked on, and values while the
+            // next scores are: the same registers, refilled as soon as their contents are used.
+            typename A::RawK rk;
+            typename A::RawV rv;
+            bool have = false, fresh = true;
+#pragma unroll 1
+            while (true) {
+                float sc[NT][4];
+                bool more = true, ends = false;
+                const Group now = s;
+                int next = x, valid = 0;
+                if (have) {
+                    A::scores(st, qs, rk, a, sc, lane);
+                    ends = ++tile == nt;
+                    next = x + 1 + (ends ? kStart : 0);
+                    more = next < xe;
+                    valid = u.valid;
+                    fresh = ends;
+                    if (ends && more) next_group(s, nt, tile);
+                }
+                if (more) {
+                    if (fresh) u.begin(c, s.b, s.h, checked_length(c, s.b), tile, lane); else u.advance(c, s.b, s.h, lane);
+                    A::load_k(rk, c, u, lane);
+                }
+                if (have) {
+                    A::probabilities(st, sc, a, x, valid, lane);
+                    A::accumulate(st, rv, sc);
+                    x = next;
+                    if (ends || !more) flush(now, ends);
+                }
+                if (!more) break;
+                if (fresh) {
+                    whole = tile == 0;
+                    A::begin(st, qs, a, s.b, head0_of(s), heads_of(s), lane);
+                    fresh = false;
+                }
+                A::load_v(rv, c, u, lane);
+                have = true;
             }
-            A::load_v(rv, c, u.v, u.vs, u.valid, lane);
-            have = true;
         }
     }
     __syncthreads();
@@ -916,7 +1027,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             float4 o;
             float top, l;
             unsigned rest = run;
-            A::template join<true>([&](int) { const int e = __ffs(rest) - 1; rest &= rest - 1; return &sm.part[e]; }, __popc(run), head, d, o, top, l);
+            A::template join<true>([&](int) { const int e = __ffs(rest) - 1; rest &= rest - 1; return e < W ? &sm.part[e] : &sm.late[e - W].part; }, __popc(run), head, d, o, top, l);
             if (whole) {
                 A::store_joined(a, s.b, head0_of(s) + head, d, o, top, l);
             } else {
