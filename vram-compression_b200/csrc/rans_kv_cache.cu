@@ -1,8 +1,10 @@
 // Paged key-value cache: appending tokens, reading them back, and eviction by
 // accumulated attention weight.  All three are bound by the rows they move.
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp4.h>
@@ -21,6 +23,7 @@ constexpr int kThreads = 256;
 
 struct RowArgs {
     RansKvCache c;
+    Divider page, heads;
     const char* k_in;
     const char* v_in;
     int64_t k_token, k_head, v_token, v_head;      // bytes
@@ -29,36 +32,83 @@ struct RowArgs {
     const int32_t* starts;
     int tokens;
     int given;
+    int part_shift;                                // log2 of a row's threads
 };
 
-// The sequence that row `token` belongs to, or -1, and the row's number within it.
-__device__ __forceinline__ int sequence_of(const RowArgs& a, int token, int& number) {
-    if (a.starts == nullptr) {
-        number = 0;
-        return token < a.c.batch ? token : -1;
-    }
-    int lo = 0, hi = a.c.batch;                    // starts[lo] <= token < starts[hi]
-    if (token < a.starts[0] || token >= a.starts[a.c.batch]) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.starts[mid] <= token) lo = mid; else hi = mid;
-    }
-    number = token - a.starts[lo];
-    return lo;
-}
+// Tokens of a block: a warp each to find out where they are.
+constexpr int kTokens = kThreads / 32;
+
+struct Where {
+    int page, slot;            // page -1: nowhere
+    int b, position;
+};
 
 __device__ __forceinline__ int rows_of(const RowArgs& a, int b) {
     return a.starts == nullptr ? 1 : max(a.starts[b + 1] - a.starts[b], 0);
 }
 
-__device__ __forceinline__ void load8(float (&x)[8], const char* p, int given) {
+// The sequence b with starts[b] <= token < starts[b + 1], by the 32 lanes of a warp, or -1.
+__device__ __forceinline__ int sequence_of(const RowArgs& a, int token, int lane) {
+    if (a.starts == nullptr) return token < a.c.batch ? token : -1;
+    const int edge = a.starts[lane == 0 ? 0 : a.c.batch];
+    if (__any_sync(~0u, lane == 0 ? token < edge : token >= edge)) return -1;
+    int lo = 0, hi = a.c.batch;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned below = __ballot_sync(~0u, at < hi && a.starts[min(at, hi)] <= token);
+        lo += (31 - __clz(below)) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
+// Where the block's tokens lie, or are to lie: `last` 0 for tokens that follow what is there, 1 for the last ones there.
+__device__ __forceinline__ void find_tokens(const RowArgs& a, Where* where, bool last) {
+    const RansKvCache& c = a.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x * kTokens + warp;
+    if (token < a.tokens) {
+        const int b = sequence_of(a, token, lane);
+        if (lane == 0) {
+            Where w{-1, 0, b, 0};
+            if (b < 0) {
+                raise(c, RANS_KV_BAD_STARTS);
+            } else {
+                const int number = a.starts == nullptr ? 0 : token - a.starts[b];
+                const int place = checked_length(c, b) + number - (last ? rows_of(a, b) : 0);
+                w.position = c.seen[b] + number;
+                if (place < 0) {
+                    raise(c, RANS_KV_BAD_STARTS);
+                } else if (place >= (int64_t)c.table_cols * c.page) {
+                    raise(c, RANS_KV_BAD_LENGTH);
+                } else {
+                    const int in_page = a.page(place);
+                    w.page = checked_page(c, b, in_page);
+                    w.slot = place - in_page * c.page;
+                }
+            }
+            where[warp] = w;
+        }
+    }
+    __syncthreads();
+}
+
+// 8 values as they are given: 16 bytes, or 32 of fp32.
+struct Given8 {
+    uint4 w[2];
+};
+
+__device__ __forceinline__ void load8(Given8& x, const char* p, int given) {
+    x.w[0] = __ldg(reinterpret_cast<const uint4*>(p));
+    if (given == RANS_KV_FP32) x.w[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+}
+
+__device__ __forceinline__ void to_float(float (&x)[8], const Given8& y, int given) {
+    const uint32_t u[8] = {y.w[0].x, y.w[0].y, y.w[0].z, y.w[0].w, y.w[1].x, y.w[1].y, y.w[1].z, y.w[1].w};
     if (given == RANS_KV_FP32) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
         return;
     }
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = given == RANS_KV_FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&u[i]))
@@ -106,58 +156,54 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& byt
 }
 
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ RowArgs a) {
+    __shared__ Where where[kTokens];
     const RansKvCache& c = a.c;
-    const int per_row = c.dim / 8;
-    const int64_t all = (int64_t)a.tokens * c.kv_heads * per_row;
-    // dim / 8 is a multiple of 8, so the 4 lanes of a block are in or out of range together
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i - (threadIdx.x & 31) < all; i += (int64_t)gridDim.x * kThreads) {
-        const int part = (int)(i % per_row);
-        const int64_t row = i / per_row;
-        const int h = (int)(row % c.kv_heads), token = (int)(row / c.kv_heads);
-        const bool in = i < all;
-        int number = 0, p = -1, slot = 0, place = 0, b = -1;
-        if (in) {
-            b = sequence_of(a, token, number);
-            if (b < 0) {
-                raise(c, RANS_KV_BAD_STARTS);
+    find_tokens(a, where, false);
+    const int per_row = 1 << a.part_shift, tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens);
+    const int all = (tokens * c.kv_heads) << a.part_shift;
+    constexpr int kAtOnce = 2;
+    // (a row has 8 threads or more, so the four lanes of a block of 32 values are in or out of range together)
+    for (int i0 = threadIdx.x; i0 - (int)(threadIdx.x & 31) < all; i0 += kThreads * kAtOnce) {
+        Given8 in[kAtOnce][2];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
+            if (i < all) {
+                const int64_t token = blockIdx.x * kTokens + t, at = (int64_t)part * (a.given == RANS_KV_FP32 ? 32 : 16);
+                load8(in[u][0], a.k_in + token * a.k_token + h * a.k_head + at, a.given);
+                load8(in[u][1], a.v_in + token * a.v_token + h * a.v_head + at, a.given);
             } else {
-                place = checked_length(c, b) + number;
-                if (place >= (int64_t)c.table_cols * c.page) {
-                    raise(c, RANS_KV_BAD_LENGTH);
-                } else {
-                    p = checked_page(c, b, place / c.page);
-                    slot = place % c.page;
-                }
+                in[u][0] = in[u][1] = Given8{};
             }
         }
-        float x[8];
-        uint32_t byte;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const char* src = w == 0 ? a.k_in + token * a.k_token + h * a.k_head : a.v_in + token * a.v_token + h * a.v_head;
-            if (in) {
-                load8(x, src + (int64_t)part * (a.given == RANS_KV_FP32 ? 32 : 16), a.given);
-            } else {
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
+            const Where w = where[i < all ? t : 0];
+            const bool stored = i < all && w.page >= 0;
+            const int64_t place = ((int64_t)w.page * c.kv_heads + h) * c.page + w.slot;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-            }
-            char* base = static_cast<char*>(w == 0 ? c.k : c.v);
-            const int64_t at = (int64_t)p * (w == 0 ? c.k_page : c.v_page) + h * (w == 0 ? c.k_head : c.v_head) + slot * (w == 0 ? c.k_slot : c.v_slot);
-            if (c.kind == RANS_KV_MXFP4) {
-                const uint32_t code = quantise8(x, byte);
-                if (p >= 0) {
-                    const int n = part / 4, q = part % 4;
-                    *reinterpret_cast<uint32_t*>(base + at + q * per_row + n * 4) = code;
-                    if (q == 0) (w == 0 ? c.k_scale : c.v_scale)[(((int64_t)p * c.kv_heads + h) * c.page + slot) * (c.dim / 32) + n] = (uint8_t)byte;
+            for (int v = 0; v < 2; ++v) {
+                float x[8];
+                to_float(x, in[u][v], a.given);
+                char* base = static_cast<char*>(v == 0 ? c.k : c.v);
+                const int64_t at = w.page * (v == 0 ? c.k_page : c.v_page) + h * (v == 0 ? c.k_head : c.v_head) + w.slot * (v == 0 ? c.k_slot : c.v_slot);
+                if (c.kind == RANS_KV_MXFP4) {
+                    uint32_t byte;
+                    const uint32_t code = quantise8(x, byte);
+                    if (stored) {
+                        const int n = part / 4, q = part % 4;
+                        *reinterpret_cast<uint32_t*>(base + at + q * per_row + n * 4) = code;
+                        if (q == 0) (v == 0 ? c.k_scale : c.v_scale)[place * (c.dim / 32) + n] = (uint8_t)byte;
+                    }
+                } else if (stored) {
+                    *reinterpret_cast<uint4*>(base + at + part * 16) = pack8(x, c.kind);
                 }
-            } else if (p >= 0) {
-                *reinterpret_cast<uint4*>(base + at + part * 16) = pack8(x, c.kind);
             }
-        }
-        if (p >= 0 && part == 0) {
-            const int64_t at = ((int64_t)p * c.kv_heads + h) * c.page + slot;
-            if (c.position != nullptr) c.position[at] = c.seen[b] + number;
-            if (c.weight != nullptr) c.weight[at] = 0.0f;
+            if (stored && part == 0) {
+                if (c.position != nullptr) c.position[place] = w.position;
+                if (c.weight != nullptr) c.weight[place] = 0.0f;
+            }
         }
     }
     // The last block to get here (all have read the lengths by then) moves them on.
@@ -179,71 +225,84 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 }
 
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ RowArgs a) {
+    __shared__ Where where[kTokens];
     const RansKvCache& c = a.c;
-    const int per_row = c.dim / 8;
-    const int64_t all = (int64_t)a.tokens * c.kv_heads * per_row;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads) {
-        const int part = (int)(i % per_row);
-        const int64_t row = i / per_row;
-        const int h = (int)(row % c.kv_heads), token = (int)(row / c.kv_heads);
-        int number = 0, p = -1, slot = 0;
-        const int b = sequence_of(a, token, number);
-        if (b < 0) {
-            raise(c, RANS_KV_BAD_STARTS);
-        } else {
-            const int place = checked_length(c, b) - rows_of(a, b) + number;
-            if (place < 0) {
-                raise(c, RANS_KV_BAD_STARTS);
-            } else {
-                p = checked_page(c, b, place / c.page);
-                slot = place % c.page;
+    find_tokens(a, where, true);
+    const int per_row = 1 << a.part_shift, tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens);
+    const int all = (tokens * c.kv_heads) << a.part_shift;
+    const int64_t out0 = ((int64_t)blockIdx.x * kTokens * c.kv_heads) << a.part_shift;
+    constexpr int kAtOnce = 2;
+    for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kAtOnce) {
+        uint4 x[kAtOnce][2];               // 4 bits: the codes in .x, the scale byte in .y
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
+            x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
+            if (i >= all) continue;
+            const Where w = where[t];
+            if (w.page < 0) continue;
+            const int64_t place = ((int64_t)w.page * c.kv_heads + h) * c.page + w.slot;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const char* base = static_cast<const char*>(v == 0 ? c.k : c.v) + w.page * (v == 0 ? c.k_page : c.v_page) +
+                                   h * (v == 0 ? c.k_head : c.v_head) + w.slot * (v == 0 ? c.k_slot : c.v_slot);
+                if (c.kind == RANS_KV_MXFP4) {
+                    x[u][v].x = *reinterpret_cast<const uint32_t*>(base + part % 4 * per_row + part / 4 * 4);
+                    x[u][v].y = (v == 0 ? c.k_scale : c.v_scale)[place * (c.dim / 32) + part / 4];
+                } else {
+                    x[u][v] = *reinterpret_cast<const uint4*>(base + part * 16);
+                }
             }
         }
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const char* base = static_cast<const char*>(w == 0 ? c.k : c.v);
-            const int64_t at = (int64_t)p * (w == 0 ? c.k_page : c.v_page) + h * (w == 0 ? c.k_head : c.v_head) + slot * (w == 0 ? c.k_slot : c.v_slot);
-            uint4 out = make_uint4(0, 0, 0, 0);
-            if (p >= 0) {
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kThreads;
+            if (i >= all) continue;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                uint4 out = x[u][v];
                 if (c.kind == RANS_KV_MXFP4) {
-                    const int n = part / 4, q = part % 4;
-                    const uint32_t code = *reinterpret_cast<const uint32_t*>(base + at + q * per_row + n * 4);
-                    const uint32_t byte = (w == 0 ? c.k_scale : c.v_scale)[(((int64_t)p * c.kv_heads + h) * c.page + slot) * (c.dim / 32) + n];
-                    const float f = byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
-                    float x[8];
+                    const float f = out.y == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(out.y << 23);
+                    float y[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const __half2_raw r = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((code >> (8 * e)) & 255), __NV_E2M1);
-                        const float2 y = __half22float2(__half2(r));
-                        x[2 * e] = y.x * f;
-                        x[2 * e + 1] = y.y * f;
+                        const __half2_raw r = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((out.x >> (8 * e)) & 255), __NV_E2M1);
+                        const float2 z = __half22float2(__half2(r));
+                        y[2 * e] = z.x * f;
+                        y[2 * e + 1] = z.y * f;
                     }
-                    out = pack8(x, RANS_KV_BF16);
-                } else {
-                    out = *reinterpret_cast<const uint4*>(base + at + part * 16);
+                    out = pack8(y, RANS_KV_BF16);
                 }
+                (v == 0 ? a.k_out : a.v_out)[out0 + i] = out;
             }
-            (w == 0 ? a.k_out : a.v_out)[i] = out;
         }
     }
 }
 
 // ------------------------------------------------------------------ evict
-// Per (sequence, kv head): find the key T of the budget-th heaviest token by
-// radix selection over 32-bit keys, mark what stays, and list the moves
-// (i-th kept place >= budget -> i-th freed place < budget).  A second kernel
-// copies the listed rows: sources lie at or above the budget and destinations
-// below it, so moves never meet.
+// Per (sequence, kv head) a cluster of blocks: find the key of the budget-th heaviest token by radix selection over 32-bit
+// keys (passes of 11, 11 and 10 bits, of which the last is seldom needed; the blocks' histograms are added up through the
+// cluster's shared memory), mark what stays, pair
+// the i-th kept place at or above the budget with the i-th freed place below it, and move the rows.  Sources lie at or above
+// the budget and destinations below it, so moves never meet.
 
 constexpr int kSelect = 1024;
 constexpr int kSelectWarps = kSelect / 32;
+constexpr int kBins = 2048;                                // two per thread
+constexpr int kMaxCluster = 8;                             // the portable size; of 16, seven at most run at a time
+constexpr int kPlaces = 4096;                              // a block takes before there are more of them
+constexpr int kMaxSharedKeys = 40 * 1024;                  // of a block; more are kept in the workspace
 
 struct EvictArgs {
     RansKvCache c;
+    Divider page;
     int budget, recent;
-    int* moves;                  // [batch * kv_heads]: number of moves
-    int2* list;                  // [batch * kv_heads][budget]: (to, from)
-    uint32_t* keys;              // [batch * kv_heads][table_cols * page]
+    int* counter;                // [batch], zero between calls
+    int* to;                     // [batch * kv_heads][budget]: place of each move's destination
+    int* from;                   // and source
+    uint32_t* keys;              // [batch * kv_heads][table_cols * page], or NULL: in shared memory
+    int* moves;                  // [batch * kv_heads]: how many, for move_kernel, or NULL: moved here
+    int row_shift;               // log2 of the 16-byte pieces of a row
 };
 
 // Order-preserving key of a weight; the newest tokens come first, then NaN.
@@ -254,160 +313,280 @@ __device__ __forceinline__ uint32_t key_of(float w, bool late) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelect) select_kernel(const __grid_constant__ EvictArgs a) {
+__device__ __forceinline__ int warp_sum(int x) { return __reduce_add_sync(~0u, x); }
+
+// Moves m0 .. m1 - 1 of one (sequence, kv head), by a block of THREADS threads.
+template <int THREADS>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, const int* to, const int* from, int m0, int m1, int4* moving) {
     const RansKvCache& c = a.c;
-    const int h = blockIdx.x % c.kv_heads, b = blockIdx.x / c.kv_heads;
+    const int tid = threadIdx.x;
+            for (int m = m0; m < m1; m += THREADS) {
+                // a thread per move: its pages, and what goes with the rows
+                const int here = min(THREADS, m1 - m);
+                if (tid < here) {
+                    const int to_t = to[m + tid], from_t = from[m + tid];
+                    const int to_page = a.page(to_t), from_page = a.page(from_t);
+            const int4 mv = make_int4(checked_page(c, b, to_page), to_t - to_page * c.page, checked_page(c, b, from_page), from_t - from_page * c.page);
+                    moving[tid] = mv;
+                    if (mv.x >= 0 && mv.z >= 0) {
+                        const int64_t x = ((int64_t)mv.x * c.kv_heads + h) * c.page + mv.y, y = ((int64_t)mv.z * c.kv_heads + h) * c.page + mv.w;
+                        c.weight[x] = c.weight[y];
+                        c.position[x] = c.position[y];
+                        if (c.kind == RANS_KV_MXFP4) {
+                            if (c.dim == 64) {
+                                reinterpret_cast<uint16_t*>(c.k_scale)[x] = reinterpret_cast<uint16_t*>(c.k_scale)[y];
+                                reinterpret_cast<uint16_t*>(c.v_scale)[x] = reinterpret_cast<uint16_t*>(c.v_scale)[y];
+                            } else if (c.dim == 128) {
+                                reinterpret_cast<uint32_t*>(c.k_scale)[x] = reinterpret_cast<uint32_t*>(c.k_scale)[y];
+                                reinterpret_cast<uint32_t*>(c.v_scale)[x] = reinterpret_cast<uint32_t*>(c.v_scale)[y];
+                            } else {
+                                reinterpret_cast<uint64_t*>(c.k_scale)[x] = reinterpret_cast<uint64_t*>(c.k_scale)[y];
+                                reinterpret_cast<uint64_t*>(c.v_scale)[x] = reinterpret_cast<uint64_t*>(c.v_scale)[y];
+                            }
+                        }
+                    }
+                }
+                __syncthreads();
+                const int all = here << (a.row_shift + 1);                       // pieces of the key and value rows
+                constexpr int kAtOnce = 4;
+                for (int i0 = tid; i0 < all; i0 += THREADS * kAtOnce) {
+                    uint4 x[kAtOnce];
+                    char* dst[kAtOnce];
+    #pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u) {
+                        const int i = i0 + u * THREADS, part = i & ((1 << a.row_shift) - 1);
+                        const bool is_k = (i >> a.row_shift & 1) == 0;
+                        dst[u] = nullptr;
+                        if (i >= all) continue;
+                        const int4 mv = moving[i >> (a.row_shift + 1)];
+                        if (mv.x < 0 || mv.z < 0) continue;                      // (a bad page: reported above)
+                        char* base = static_cast<char*>(is_k ? c.k : c.v) + h * (is_k ? c.k_head : c.v_head) + part * 16;
+                        const int64_t page = is_k ? c.k_page : c.v_page, slot = is_k ? c.k_slot : c.v_slot;
+                        x[u] = *reinterpret_cast<const uint4*>(base + mv.z * page + mv.w * slot);
+                        dst[u] = base + mv.x * page + mv.y * slot;
+                    }
+    #pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+                        if (dst[u] != nullptr) *reinterpret_cast<uint4*>(dst[u]) = x[u];
+                }
+                __syncthreads();
+            }
+}
+
+__global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ EvictArgs a) {
+    extern __shared__ uint32_t shared_keys[];
+    __shared__ __align__(8) int hist[2][kBins];
+    __shared__ int digit_s, rank_s, count_s;
+    __shared__ int wsum[2][kSelectWarps];
+    __shared__ int block_sum[3];                           // ties, holes, movers of the block's places
+    __shared__ int4 moving[kSelect];                       // (page, slot) to and from
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const RansKvCache& c = a.c;
+    const int blocks = cluster.num_blocks(), block = cluster.block_rank(), bh = blockIdx.x / blocks;
+    const int h = bh % c.kv_heads, b = bh / c.kv_heads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    __shared__ int hist[256];
-    __shared__ int digit_s, rank_s;
-    __shared__ int wsum[kSelectWarps + 1], wsum2[kSelectWarps + 1];
     const int n = checked_length(c, b), k = a.budget;
-    if (n <= k) {
-        if (tid == 0) a.moves[blockIdx.x] = 0;
-        return;
-    }
-    uint32_t* keys = a.keys + (int64_t)blockIdx.x * c.table_cols * c.page;
-    const int first_late = c.seen[b] - a.recent;
-    for (int t = tid; t < n; t += kSelect) {
-        const int p = checked_page(c, b, t / c.page);
-        uint32_t key = 0;
-        if (p >= 0) {
-            const int64_t at = ((int64_t)p * c.kv_heads + h) * c.page + t % c.page;
-            key = key_of(c.weight[at], c.position[at] >= first_late);
+    if (n > k) {
+        // each block has a run of 32-place words, each warp a run of the block's
+        const int words = (n + 31) / 32, bw0 = (int)((int64_t)words * block / blocks), bw1 = (int)((int64_t)words * (block + 1) / blocks);
+        const int w0 = bw0 + (bw1 - bw0) * warp / kSelectWarps, w1 = bw0 + (bw1 - bw0) * (warp + 1) / kSelectWarps;
+        uint32_t* keys = a.keys != nullptr ? a.keys + (int64_t)bh * c.table_cols * c.page : shared_keys - (int64_t)bw0 * 32;
+        const int first_late = c.seen[b] - a.recent;
+        const int t_end = min(bw1 * 32, n);
+        constexpr int kLoads = 4;
+        for (int t0 = bw0 * 32 + tid; t0 < t_end; t0 += kSelect * kLoads) {
+            int64_t at[kLoads];
+            float weight[kLoads];
+            int position[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int t = t0 + i * kSelect, in_page = a.page(t), p = t < t_end ? checked_page(c, b, in_page) : -1;
+                at[i] = p >= 0 ? ((int64_t)p * c.kv_heads + h) * c.page + (t - in_page * c.page) : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                weight[i] = at[i] >= 0 ? c.weight[at[i]] : 0.0f;
+                position[i] = at[i] >= 0 ? c.position[at[i]] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (t0 + i * kSelect < t_end) keys[t0 + i * kSelect] = at[i] >= 0 ? key_of(weight[i], position[i] >= first_late) : 0;
         }
-        keys[t] = key;
-    }
-    __syncthreads();
-    uint32_t prefix = 0;
-    int rank = k;                                          // of the threshold among the keys that share the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelect) hist[i] = 0;
-        __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int t = tid; t < n; t += kSelect) {
-            const uint32_t key = keys[t];
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (warp == 0) {
-            // lane l: digits 255 - 8 l downwards
-            int own = 0;
-            for (int i = 0; i < 8; ++i) own += hist[255 - 8 * lane - i];
-            int inc = own;
+        uint32_t prefix = 0;
+        int rank = k;                                      // of the threshold among the keys that share the prefix
+        auto sync = [&]() {
+            if (blocks == 1) __syncthreads(); else cluster.sync();
+        };
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t mask = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;        // of the digits found
+            int* mine = hist[pass & 1];
+            mine[tid] = mine[tid + kSelect] = 0;
+            __syncthreads();
+            for (int w = w0; w < w1; ++w) {
+                const int t = w * 32 + lane;
+                const uint32_t key = t < n ? keys[t] : 0;
+                if (t < n && (key & mask) == prefix) atomicAdd(&mine[(key >> shift) & (kBins - 1)], 1);
+            }
+            sync();
+            // thread i: the bins kBins - 1 - 2 i and the one below, of all blocks
+            int2 sum = make_int2(0, 0);
+            for (int r = 0; r < blocks; ++r) {
+                const int2 x = reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r))[kSelect - 1 - tid];
+                sum.x += x.y;
+                sum.y += x.x;
+            }
+            int inc = sum.x + sum.y;
 #pragma unroll
             for (int i = 1; i < 32; i *= 2) {
                 const int y = __shfl_up_sync(~0u, inc, i);
                 if (lane >= i) inc += y;
             }
-            int before = inc - own;
-            if (before < rank && rank <= inc)
-                for (int i = 0; i < 8; ++i) {
-                    const int d = 255 - 8 * lane - i;
-                    if (rank <= before + hist[d]) { digit_s = d; rank_s = rank - before; break; }
-                    before += hist[d];
-                }
+            if (lane == 31) wsum[pass & 1][warp] = inc;
+            __syncthreads();
+            const int before = inc - sum.x - sum.y + warp_sum(lane < warp ? wsum[pass & 1][lane] : 0);
+            if (before < rank && rank <= before + sum.x + sum.y) {
+                const bool second = rank > before + sum.x;
+                digit_s = kBins - 1 - 2 * tid - (second ? 1 : 0);
+                rank_s = rank - before - (second ? sum.x : 0);
+                count_s = second ? sum.y : sum.x;
+            }
+            __syncthreads();
+            prefix |= (uint32_t)digit_s << shift;
+            rank = rank_s;
+            if (rank == count_s) {
+                // all that share these digits stay: no ties to part.  (prefix > 0, for n > budget keys are not all kept.)
+                --prefix;
+                rank = 0;
+                break;
+            }
+        }
+        // Keys above `prefix` stay, and the first `rank` places whose key equals it.
+        int tie0 = 0;
+        if (rank > 0) {
+            int ties = 0;
+            for (int w = w0; w < w1; ++w) {
+                const int t = w * 32 + lane;
+                ties += __popc(__ballot_sync(~0u, t < n && keys[t] == prefix));
+            }
+            __syncthreads();
+            if (lane == 0) wsum[0][warp] = ties;
+            __syncthreads();
+            tie0 = warp_sum(lane < warp ? wsum[0][lane] : 0);
+            if (tid == kSelect - 1) block_sum[0] = tie0 + ties;
+            sync();
+            tie0 += warp_sum(lane < block ? *cluster.map_shared_rank(&block_sum[0], lane) : 0);
+        }
+        auto kept = [&](int w, int& tie) {
+            const int t = w * 32 + lane;
+            const uint32_t key = t < n ? keys[t] : 0;
+            const unsigned equal = __ballot_sync(~0u, t < n && key == prefix);
+            const bool keep = t < n && (key > prefix || (key == prefix && tie + __popc(equal & ((1u << lane) - 1)) < rank));
+            tie += __popc(equal);
+            return keep;
+        };
+        int holes = 0, movers = 0, tie = tie0;
+        for (int w = w0; w < w1; ++w) {
+            const int t = w * 32 + lane;
+            const bool keep = kept(w, tie);
+            holes += __popc(__ballot_sync(~0u, t < k && !keep));
+            movers += __popc(__ballot_sync(~0u, t >= k && keep));
         }
         __syncthreads();
-        prefix |= (uint32_t)digit_s << shift;
-        rank = rank_s;
+        if (lane == 0) {
+            wsum[0][warp] = holes;
+            wsum[1][warp] = movers;
+        }
+        __syncthreads();
+        int hole = warp_sum(lane < warp ? wsum[0][lane] : 0), mover = warp_sum(lane < warp ? wsum[1][lane] : 0);
+        if (tid == kSelect - 1) {
+            block_sum[1] = hole + holes;
+            block_sum[2] = mover + movers;
+        }
+        sync();
+        const int block_holes = lane < blocks ? *cluster.map_shared_rank(&block_sum[1], lane) : 0;
+        const int block_movers = lane < blocks ? *cluster.map_shared_rank(&block_sum[2], lane) : 0;
+        hole += warp_sum(lane < block ? block_holes : 0);
+        mover += warp_sum(lane < block ? block_movers : 0);
+        const int moves = warp_sum(block_holes);
+        int *to = a.to + (int64_t)bh * k, *from = a.from + (int64_t)bh * k;
+        tie = tie0;
+        for (int w = w0; w < w1; ++w) {
+            const int t = w * 32 + lane;
+            const bool keep = kept(w, tie);
+            const unsigned is_hole = __ballot_sync(~0u, t < k && !keep), is_mover = __ballot_sync(~0u, t >= k && keep);
+            const unsigned below = (1u << lane) - 1;
+            if (is_hole >> lane & 1) to[hole + __popc(is_hole & below)] = t;
+            if (is_mover >> lane & 1) from[mover + __popc(is_mover & below)] = t;
+            hole += __popc(is_hole);
+            mover += __popc(is_mover);
+        }
+        sync();                                            // the lists are whole; nobody reads another block's memory from here on
+
+        if (a.moves != nullptr) {
+            if (block == 0 && tid == 0) a.moves[bh] = moves;
+        } else {
+            move_rows<kSelect>(a, b, h, to, from, (int)((int64_t)moves * block / blocks), (int)((int64_t)moves * (block + 1) / blocks), moving);
+        }
+    } else if (a.moves != nullptr && block == 0 && tid == 0) {
+        a.moves[bh] = 0;
     }
-    // Keys above `prefix` stay, and the first `rank` that equal it.  Each warp has a run of places.
-    const int words = (n + 31) / 32, w0 = (int)((int64_t)words * warp / kSelectWarps), w1 = (int)((int64_t)words * (warp + 1) / kSelectWarps);
-    int ties = 0;
-    for (int w = w0; w < w1; ++w) {
-        const int t = w * 32 + lane;
-        ties += __popc(__ballot_sync(~0u, t < n && keys[t] == prefix));
-    }
-    if (lane == 0) wsum[warp] = ties;
+    // The last block of a sequence (all have read its length by then) shortens it.
     __syncthreads();
-    int tie0 = 0;
-    for (int w = 0; w < warp; ++w) tie0 += wsum[w];
-    __syncthreads();
-    auto kept = [&](int w, int& tie) {
-        const int t = w * 32 + lane;
-        const uint32_t key = t < n ? keys[t] : 0;
-        const unsigned equal = __ballot_sync(~0u, t < n && key == prefix);
-        const bool keep = t < n && (key > prefix || (key == prefix && tie + __popc(equal & ((1u << lane) - 1)) < rank));
-        tie += __popc(equal);
-        return keep;
-    };
-    int holes = 0, movers = 0, tie = tie0;
-    for (int w = w0; w < w1; ++w) {
-        const int t = w * 32 + lane;
-        const bool keep = kept(w, tie);
-        holes += __popc(__ballot_sync(~0u, t < k && !keep));
-        movers += __popc(__ballot_sync(~0u, t >= k && keep));
+    if (tid == 0) {
+        __threadfence();
+        if (atomicAdd(a.counter + b, 1) == blocks * c.kv_heads - 1) {
+            a.counter[b] = 0;
+            if (n > k) c.length[b] = k;
+        }
     }
-    if (lane == 0) { wsum[warp] = holes; wsum2[warp] = movers; }
-    __syncthreads();
-    int hole = 0, mover = 0;
-    for (int w = 0; w < warp; ++w) { hole += wsum[w]; mover += wsum2[w]; }
-    int2* list = a.list + (int64_t)blockIdx.x * a.budget;
-    tie = tie0;
-    for (int w = w0; w < w1; ++w) {
-        const int t = w * 32 + lane;
-        const bool keep = kept(w, tie);
-        const unsigned is_hole = __ballot_sync(~0u, t < k && !keep), is_mover = __ballot_sync(~0u, t >= k && keep);
-        const unsigned below = (1u << lane) - 1;
-        if (is_hole >> lane & 1) list[hole + __popc(is_hole & below)].x = t;
-        if (is_mover >> lane & 1) list[mover + __popc(is_mover & below)].y = t;
-        hole += __popc(is_hole);
-        mover += __popc(is_mover);
-    }
-    if (tid == kSelect - 1) a.moves[blockIdx.x] = mover;
 }
 
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ EvictArgs a) {
-    const RansKvCache& c = a.c;
-    const int bh = blockIdx.y, h = bh % c.kv_heads, b = bh / c.kv_heads;
-    const int count = a.moves[bh];
-    const int2* list = a.list + (int64_t)bh * a.budget;
-    const int row = c.kind == RANS_KV_MXFP4 ? c.dim / 32 : c.dim / 8;      // 16-byte pieces of a row
-    const int64_t all = (int64_t)count * row;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads) {
-        const int m = (int)(i / row), part = (int)(i % row);
-        const int2 move = list[m];
-        const int pt = checked_page(c, b, move.x / c.page), pf = checked_page(c, b, move.y / c.page);
-        if (pt < 0 || pf < 0) continue;
-        const int st = move.x % c.page, sf = move.y % c.page;
-        const char* k = static_cast<const char*>(c.k) + h * c.k_head + part * 16;
-        const char* v = static_cast<const char*>(c.v) + h * c.v_head + part * 16;
-        const uint4 x = *reinterpret_cast<const uint4*>(k + pf * c.k_page + sf * c.k_slot);
-        const uint4 y = *reinterpret_cast<const uint4*>(v + pf * c.v_page + sf * c.v_slot);
-        *reinterpret_cast<uint4*>(const_cast<char*>(k) + pt * c.k_page + st * c.k_slot) = x;
-        *reinterpret_cast<uint4*>(const_cast<char*>(v) + pt * c.v_page + st * c.v_slot) = y;
-        const int64_t to = ((int64_t)pt * c.kv_heads + h) * c.page + st, from = ((int64_t)pf * c.kv_heads + h) * c.page + sf;
-        if (c.kind == RANS_KV_MXFP4) {
-            c.k_scale[to * row + part] = c.k_scale[from * row + part];     // dim / 32 scale bytes, as many as pieces
-            c.v_scale[to * row + part] = c.v_scale[from * row + part];
-        }
-        if (part == 0) {
-            c.weight[to] = c.weight[from];
-            c.position[to] = c.position[from];
-        }
-    }
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) c.length[b] = min(checked_length(c, b), a.budget);
+    __shared__ int4 moving[kThreads];
+    const int bh = blockIdx.y, moves = a.moves[bh];
+    const int m0 = (int)((int64_t)moves * blockIdx.x / gridDim.x), m1 = (int)((int64_t)moves * (blockIdx.x + 1) / gridDim.x);
+    move_rows<kThreads>(a, bh / a.c.kv_heads, bh % a.c.kv_heads, a.to + (int64_t)bh * a.budget, a.from + (int64_t)bh * a.budget, m0, m1, moving);
 }
 
 struct EvictPlan {
-    int64_t moves, list, keys, bytes;
+    int64_t to, from, moves, keys, bytes;
+    bool apart;                      // moves in a kernel of their own
+    int blocks, shared_keys;         // of a (sequence, kv head); keys a block holds in shared memory (0: in the workspace)
 };
 
 bool plan_evict(const RansKvCache& c, int budget, EvictPlan& p) {
     if (budget < 1) return false;
     auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
-    const int64_t heads = (int64_t)c.batch * c.kv_heads;
-    p.moves = counter_bytes(c);
-    p.list = p.moves + up(heads * 4);
-    p.keys = p.list + up(heads * budget * 8);
-    p.bytes = p.keys + up(heads * c.table_cols * c.page * 4);
+    const int64_t heads = (int64_t)c.batch * c.kv_heads, room = (int64_t)c.table_cols * c.page;
+    // as many blocks as fill the SMs once, but no more than have a few places for each thread
+    p.blocks = 1;
+    while (p.blocks < kMaxCluster && heads * p.blocks * 2 <= kSms && room > (int64_t)p.blocks * kPlaces) p.blocks *= 2;
+    const int64_t most = ((room + 31) / 32 / p.blocks + 1) * 32;
+    p.shared_keys = most <= kMaxSharedKeys ? (int)most : 0;
+    p.to = counter_bytes(c);
+    p.from = p.to + up(heads * budget * 4);
+    p.moves = p.from + up(heads * budget * 4);
+    p.keys = p.moves + up(heads * 4);
+    // Few heads leave SMs without a block of the selection: from 32 MB on, the moves get a grid of their own.
+    const int64_t row = c.kind == RANS_KV_MXFP4 ? c.dim / 2 : c.dim * 2, most_moves = room > budget ? (budget < room - budget ? budget : room - budget) : 0;
+    p.apart = heads * p.blocks < kSms && heads * most_moves * row * 2 >= (32 << 20);
+    p.bytes = p.keys + (p.shared_keys ? 0 : up(heads * room * 4));
     return true;
 }
 
-int row_grid(const RowArgs& a) {
-    const int64_t blocks = ((int64_t)a.tokens * a.c.kv_heads * (a.c.dim / 8) + kThreads - 1) / kThreads;
-    return (int)(blocks < kSms * 8 ? blocks : kSms * 8);
+void set_rows(RowArgs& a, const RansKvCache& c, const int32_t* starts, int tokens) {
+    a.c = c;
+    fill_strides(a.c);
+    a.page = Divider::of((uint32_t)c.page);
+    a.heads = Divider::of((uint32_t)c.kv_heads);
+    a.starts = starts;
+    a.tokens = tokens;
+    a.part_shift = c.dim == 64 ? 3 : c.dim == 128 ? 4 : 5;
 }
+
+int row_grid(const RowArgs& a) { return (a.tokens + kTokens - 1) / kTokens; }
 
 }  // namespace
 }  // namespace rb200kv
@@ -423,13 +602,10 @@ extern "C" int rans_kv_append(const RansKvCache* cache, const void* k, const voi
     if (tokens == 0) return 0;
     if (k == nullptr || v == nullptr || !aligned16(k) || !aligned16(v) || ((k_token | k_head | v_token | v_head) & 15)) return -2;
     RowArgs a{};
-    a.c = *cache;
-    fill_strides(a.c);
+    set_rows(a, *cache, starts, tokens);
     a.k_in = static_cast<const char*>(k);
     a.v_in = static_cast<const char*>(v);
     a.k_token = k_token; a.k_head = k_head; a.v_token = v_token; a.v_head = v_head;
-    a.starts = starts;
-    a.tokens = tokens;
     a.given = given;
     append_kernel<<<row_grid(a), kThreads, 0, stream>>>(a);
     return (int)cudaGetLastError();
@@ -443,12 +619,9 @@ extern "C" int rans_kv_read(const RansKvCache* cache, void* k_out, void* v_out, 
     if (tokens == 0) return 0;
     if (k_out == nullptr || v_out == nullptr || !aligned16(k_out) || !aligned16(v_out)) return -2;
     RowArgs a{};
-    a.c = *cache;
-    fill_strides(a.c);
+    set_rows(a, *cache, starts, tokens);
     a.k_out = static_cast<uint4*>(k_out);
     a.v_out = static_cast<uint4*>(v_out);
-    a.starts = starts;
-    a.tokens = tokens;
     read_kernel<<<row_grid(a), kThreads, 0, stream>>>(a);
     return (int)cudaGetLastError();
 }
@@ -468,17 +641,42 @@ extern "C" int rans_kv_evict(const RansKvCache* cache, int budget, int recent, c
     EvictArgs a{};
     a.c = *cache;
     fill_strides(a.c);
+    a.page = Divider::of((uint32_t)cache->page);
     char* ws = static_cast<char*>(cache->workspace);
     a.budget = budget;
     a.recent = recent;
-    a.moves = reinterpret_cast<int*>(ws + p.moves);
-    a.list = reinterpret_cast<int2*>(ws + p.list);
-    a.keys = reinterpret_cast<uint32_t*>(ws + p.keys);
-    const int heads = cache->batch * cache->kv_heads;
-    select_kernel<<<heads, kSelect, 0, stream>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    a.counter = reinterpret_cast<int*>(ws + 256);
+    a.to = reinterpret_cast<int*>(ws + p.to);
+    a.from = reinterpret_cast<int*>(ws + p.from);
+    a.keys = p.shared_keys ? nullptr : reinterpret_cast<uint32_t*>(ws + p.keys);
+    for (int pieces = cache->kind == RANS_KV_MXFP4 ? cache->dim / 32 : cache->dim / 8; pieces > 1; pieces /= 2) ++a.row_shift;
+    a.moves = p.apart ? reinterpret_cast<int*>(ws + p.moves) : nullptr;
+    static std::atomic<uint64_t> told{0};      // per device: the kernel may use this much shared memory
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
-    const int chunks = heads >= kSms * 8 ? 1 : (kSms * 8 + heads - 1) / heads;
-    move_kernel<<<dim3(chunks, heads), kThreads, 0, stream>>>(a);
+    const uint64_t bit = (uint64_t)1 << (device & 63);
+    if ((told.load(std::memory_order_relaxed) & bit) == 0) {
+        e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4);
+        if (e != cudaSuccess) return (int)e;
+        told.fetch_or(bit, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(cache->batch * cache->kv_heads * p.blocks);
+    config.blockDim = dim3(kSelect);
+    config.dynamicSmemBytes = (size_t)p.shared_keys * 4;
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = p.blocks;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    e = cudaLaunchKernelEx(&config, evict_kernel, a);
+    if (e != cudaSuccess) return (int)e;
+    if (p.apart) {
+        const int heads = cache->batch * cache->kv_heads;
+        move_kernel<<<dim3((5 * kSms + heads - 1) / heads, heads), kThreads, 0, stream>>>(a);
+    }
     return (int)cudaGetLastError();
 }

@@ -15,6 +15,19 @@ constexpr int kMaxSubgroups = 16;        // head groups of one kv head (see rans
 
 __device__ __forceinline__ void raise(const RansKvCache& c, int bit) { atomicOr(c.status, bit); }
 
+// Division of 0 <= n < 2^31 by a fixed number: (umulhi(n, mul) + n) >> shift, with mul = floor(2^32 (2^shift - d) / d) + 1
+// and shift = ceil(log2 d).  The compiler's division is some thirty instructions, more than the rest of a page lookup.
+struct Divider {
+    uint32_t mul;
+    int shift;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+    static Divider of(uint32_t d) {
+        int shift = 0;
+        while (((uint64_t)1 << shift) < d) ++shift;
+        return {(uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1), shift};
+    }
+};
+
 // length[b] within what the table can hold; never follows a bad one.
 __device__ __forceinline__ int checked_length(const RansKvCache& c, int b) {
     const int n = c.length[b];
