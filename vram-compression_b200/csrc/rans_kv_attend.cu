@@ -54,6 +54,7 @@ constexpr float kHigh = 15.0f, kRest = 11.0f;
 
 struct AttendArgs {
     RansKvCache c;
+    Divider page;
     const char* q;
     int64_t q_batch, q_head;     // bytes
     void* out;
@@ -230,9 +231,9 @@ struct Attend {
             // only a page that holds tokens is looked up (n <= table_cols * page, so `ahead` is then inside the table)
             next = left > c.page - slot ? __ldg(c.table + (int64_t)b * c.table_cols + ahead) : -1;
         }
-        __device__ __forceinline__ void begin(const RansKvCache& c, int b, int h, int n, int tile, int lane) {
+        __device__ __forceinline__ void begin(const RansKvCache& c, const Divider& page, int b, int h, int n, int tile, int lane) {
             const int t0 = tile * kTile;
-            ahead = t0 / c.page;
+            ahead = page(t0);
             slot = t0 - ahead * c.page;
             left = n - t0;
             at_page(c, h, __ldg(c.table + (int64_t)b * c.table_cols + ahead), lane);
@@ -811,6 +812,8 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int segs = c.kv_heads * a.subs;               // groups of one sequence
 
+    wait_for_previous();
+    let_next_start();
     // Places in front of each sequence.
     {
         const int per = (c.batch + kThreads - 1) / kThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
@@ -915,7 +918,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             bool fresh = true, ahead_fresh = true;
             auto copy = [&](int stage) {
                 if (ahead_x < xe) {
-                    if (ahead_fresh) u.begin(c, ahead.b, ahead.h, checked_length(c, ahead.b), ahead_tile, lane);
+                    if (ahead_fresh) u.begin(c, a.page, ahead.b, ahead.h, checked_length(c, ahead.b), ahead_tile, lane);
                     else u.advance(c, ahead.b, ahead.h, lane);
                     valid = (valid & ~(255u << (8 * stage))) | (uint32_t)u.valid << (8 * stage);
                     A::copy_tile(stages[stage], c, u, lane);
@@ -975,7 +978,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                     if (ends && more) next_group(s, nt, tile);
                 }
                 if (more) {
-                    if (fresh) u.begin(c, s.b, s.h, checked_length(c, s.b), tile, lane); else u.advance(c, s.b, s.h, lane);
+                    if (fresh) u.begin(c, a.page, s.b, s.h, checked_length(c, s.b), tile, lane); else u.advance(c, s.b, s.h, lane);
                     A::load_k(rk, c, u, lane);
                 }
                 if (have) {
@@ -1068,59 +1071,104 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     }
 }
 
-// weight[t] += sum over the query heads of exp2(score - m) / l, one thread per token and kv head.
+// weight[t] += sum over a kv head's query heads of exp2(score - m) / l.  A warp takes 64 tokens of a head at a time, each lane
+// two of them: scores are read 32 bytes a lane, the heads' m and 1 / l by one lane each.
 constexpr int kWeighThreads = 256;
+constexpr int kSpan = 64;
+constexpr int kWeighBlocks = 6;          // an SM
 
-__global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_constant__ AttendArgs a, int hp) {
-    __shared__ int pre[RANS_KV_MAX_BATCH + 1];
-    __shared__ int warp_sum[kWeighThreads / 32];
+template <int HP>
+__global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_constant__ AttendArgs a) {
+    __shared__ int places[RANS_KV_MAX_BATCH + 1], spans[RANS_KV_MAX_BATCH + 1];      // of one head, in front of each sequence
+    __shared__ int warp_sum[2][kWeighThreads / 32];
     const RansKvCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (c.batch + kWeighThreads - 1) / kWeighThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += places_of(checked_length(c, b));
-    int inc = sum;
+    // The lengths do not change during the attention before this kernel, which began when they were complete: they may be
+    // read before it ends.
+    {
+        const int per = (c.batch + kWeighThreads - 1) / kWeighThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
+        int sum[2] = {0, 0};
+        for (int b = b0; b < b1; ++b) {
+            const int n = checked_length(c, b);
+            sum[0] += places_of(n);
+            sum[1] += (n + kSpan - 1) / kSpan;
+        }
+        int inc[2] = {sum[0], sum[1]};
 #pragma unroll
-    for (int i = 1; i < 32; i *= 2) {
-        const int y = __shfl_up_sync(~0u, inc, i);
-        if (lane >= i) inc += y;
-    }
-    if (lane == 31) warp_sum[warp] = inc;
-    __syncthreads();
-    int at = inc - sum;
-    for (int w = 0; w < warp; ++w) at += warp_sum[w];
-    for (int b = b0; b < b1; ++b) {
-        pre[b] = at;
-        at += places_of(checked_length(c, b));
-    }
-    if (b1 == c.batch && b0 < b1) pre[c.batch] = at;
-    __syncthreads();
-    const int total = pre[c.batch];                     // places of one head of every sequence, as in attend_kernel
-    const int64_t all = (int64_t)total * c.kv_heads * kTile;
-    for (int64_t i = (int64_t)blockIdx.x * kWeighThreads + tid; i < all; i += (int64_t)gridDim.x * kWeighThreads) {
-        const int64_t xt = i / kTile;                   // (sequence, kv head, place)
-        int lo = 0, hi = c.batch;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if ((int64_t)pre[mid] * c.kv_heads <= xt) lo = mid; else hi = mid;
+        for (int i = 1; i < 32; i *= 2) {
+            const int x = __shfl_up_sync(~0u, inc[0], i), y = __shfl_up_sync(~0u, inc[1], i);
+            if (lane >= i) {
+                inc[0] += x;
+                inc[1] += y;
+            }
         }
-        const int b = lo, nt = pre[b + 1] - pre[b];
-        const int64_t in = xt - (int64_t)pre[b] * c.kv_heads;
-        const int h = (int)(in / nt), tile = (int)(in - (int64_t)h * nt), t = tile * kTile + (int)(i % kTile);
-        if (t >= checked_length(c, b)) continue;
-        const int p = checked_page(c, b, t / c.page);
-        if (p < 0) continue;
-        float add = 0.0f;
+        if (lane == 31) {
+            warp_sum[0][warp] = inc[0];
+            warp_sum[1][warp] = inc[1];
+        }
+        __syncthreads();
+        int at[2] = {inc[0] - sum[0], inc[1] - sum[1]};
+        for (int w = 0; w < warp; ++w) {
+            at[0] += warp_sum[0][w];
+            at[1] += warp_sum[1][w];
+        }
+        for (int b = b0; b < b1; ++b) {
+            const int n = checked_length(c, b);
+            places[b] = at[0];
+            spans[b] = at[1];
+            at[0] += places_of(n);
+            at[1] += (n + kSpan - 1) / kSpan;
+        }
+        if (b1 == c.batch && b0 < b1) spans[c.batch] = at[1];
+        __syncthreads();
+    }
+    wait_for_previous();
+    let_next_start();
+    const int total = spans[c.batch] * c.kv_heads;
+    for (int i = blockIdx.x * (kWeighThreads / 32) + warp; i < total; i += gridDim.x * (kWeighThreads / 32)) {
+        int b = 0, hi = c.batch;
+        while (hi - b > 1) {
+            const int mid = (b + hi) / 2;
+            if (spans[mid] * c.kv_heads <= i) b = mid; else hi = mid;
+        }
+        const int per_head = spans[b + 1] - spans[b], in = i - spans[b] * c.kv_heads, h = in / per_head, t0 = (in - h * per_head) * kSpan;
+        const int n = checked_length(c, b), per_group = places_of(n);
+        int64_t at[2];
+        float add[2] = {0.0f, 0.0f}, before[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int t = t0 + e * 32 + lane, in_page = a.page(t), p = t < n ? checked_page(c, b, in_page) : -1;
+            at[e] = p >= 0 ? ((int64_t)p * c.kv_heads + h) * c.page + (t - in_page * c.page) : -1;
+        }
         for (int sub = 0; sub < a.subs; ++sub) {
-            const int64_t x = (int64_t)pre[b] * c.kv_heads * a.subs + ((int64_t)h * a.subs + sub) * nt + tile;
-            if (x >= a.score_tiles) { raise(c, RANS_KV_BAD_LENGTH); break; }
-            const float* s = a.scores + (x * kTile + i % kTile) * hp;
             const int first = sub * a.sub_heads, heads = min(a.sub_heads, a.group - first);
-            const float2* st = a.stats + (int64_t)b * a.heads + h * a.group + first;
-            for (int k = 0; k < heads; ++k) add = fmaf(exp2_fast(s[k] - st[k].x), st[k].y, add);
+            const int64_t x = (int64_t)places[b] * c.kv_heads * a.subs + (int64_t)(h * a.subs + sub) * per_group + t0 / kTile;
+            if (x + (min(t0 + kSpan, n) - 1 - t0) / kTile >= a.score_tiles) {
+                raise(c, RANS_KV_BAD_LENGTH);
+                break;
+            }
+            const float2 ml = lane < heads ? a.stats[(int64_t)b * a.heads + h * a.group + first + lane] : make_float2(0.0f, 0.0f);
+            float4 s[2][HP / 4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int k = 0; k < HP / 4; ++k)
+                    s[e][k] = at[e] >= 0 ? __ldcg(reinterpret_cast<const float4*>(a.scores + (x * kTile + e * 32 + lane) * HP) + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (sub == 0)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) before[e] = at[e] >= 0 ? c.weight[at[e]] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < HP; ++k) {
+                if (k >= heads) break;
+                const float m = __shfl_sync(~0u, ml.x, k), l = __shfl_sync(~0u, ml.y, k);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) add[e] = fmaf(exp2_fast((&s[e][k / 4].x)[k % 4] - m), l, add[e]);
+            }
+            if (sub == a.subs - 1)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (at[e] >= 0) c.weight[at[e]] = before[e] + add[e];
         }
-        float* w = c.weight + ((int64_t)p * c.kv_heads + h) * c.page + t % c.page;
-        *w += add;
     }
 }
 
@@ -1164,8 +1212,7 @@ int launch(const AttendArgs& a, cudaStream_t stream) {
         if (e != cudaSuccess) return (int)e;
         told.fetch_or(bit, std::memory_order_relaxed);
     }
-    kernel<<<kGrid, A::kWarps * 32, sizeof(typename A::Smem), stream>>>(a);
-    return (int)cudaGetLastError();
+    return launch_after(kernel, dim3(kGrid), A::kWarps * 32, sizeof(typename A::Smem), 1, stream, a);
 }
 
 template <int KIND>
@@ -1208,6 +1255,7 @@ extern "C" int rans_kv_attend(const RansKvCache* cache, const void* q, int q_kin
     AttendArgs a{};
     a.c = *cache;
     fill_strides(a.c);
+    a.page = Divider::of((uint32_t)cache->page);
     char* ws = static_cast<char*>(cache->workspace);
     a.q = static_cast<const char*>(q);
     a.q_batch = q_batch;
@@ -1233,6 +1281,5 @@ extern "C" int rans_kv_attend(const RansKvCache* cache, const void* q, int q_kin
         default: e = launch_kind<RANS_KV_MXFP4>(a, p.nt, stream); break;
     }
     if (e != 0 || !weigh) return e;
-    weigh_kernel<<<kSms * 8, kWeighThreads, 0, stream>>>(a, p.nt * 8);
-    return (int)cudaGetLastError();
+    return launch_after(p.nt == 1 ? weigh_kernel<8> : weigh_kernel<16>, dim3(kSms * kWeighBlocks), kWeighThreads, 0, 1, stream, a);
 }

@@ -31,7 +31,6 @@ struct RowArgs {
     uint4* v_out;
     const int32_t* starts;
     int tokens;
-    int given;
     int part_shift;                                // log2 of a row's threads
 };
 
@@ -47,19 +46,22 @@ __device__ __forceinline__ int rows_of(const RowArgs& a, int b) {
     return a.starts == nullptr ? 1 : max(a.starts[b + 1] - a.starts[b], 0);
 }
 
-// The sequence b with starts[b] <= token < starts[b + 1], by the 32 lanes of a warp, or -1.
-__device__ __forceinline__ int sequence_of(const RowArgs& a, int token, int lane) {
+// The sequence b with starts[b] <= token < starts[b + 1], by the 32 lanes of a warp, and its first row; -1 if there is none.
+__device__ __forceinline__ int sequence_of(const RowArgs& a, int token, int lane, int& first) {
+    first = token;
     if (a.starts == nullptr) return token < a.c.batch ? token : -1;
     const int edge = a.starts[lane == 0 ? 0 : a.c.batch];
-    if (__any_sync(~0u, lane == 0 ? token < edge : token >= edge)) return -1;
-    int lo = 0, hi = a.c.batch;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const unsigned below = __ballot_sync(~0u, at < hi && a.starts[min(at, hi)] <= token);
-        lo += (31 - __clz(below)) * step;
+    int lo = 0, hi = a.c.batch, step;
+    do {
+        step = (hi - lo + 31) / 32;
+        const int at = lo + lane * step, start = a.starts[min(at, hi)];
+        const unsigned below = __ballot_sync(~0u, at < hi && start <= token);
+        const int of = below == 0 ? 0 : 31 - __clz(below);
+        first = __shfl_sync(~0u, start, of);
+        lo += of * step;
         hi = min(lo + step, hi);
-    }
-    return lo;
+    } while (hi - lo > 1);
+    return __any_sync(~0u, lane == 0 ? token < edge : token >= edge) ? -1 : lo;
 }
 
 // Where the block's tokens lie, or are to lie: `last` 0 for tokens that follow what is there, 1 for the last ones there.
@@ -67,13 +69,14 @@ __device__ __forceinline__ void find_tokens(const RowArgs& a, Where* where, bool
     const RansKvCache& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x * kTokens + warp;
     if (token < a.tokens) {
-        const int b = sequence_of(a, token, lane);
+        int first;
+        const int b = sequence_of(a, token, lane, first);
         if (lane == 0) {
             Where w{-1, 0, b, 0};
             if (b < 0) {
                 raise(c, RANS_KV_BAD_STARTS);
             } else {
-                const int number = a.starts == nullptr ? 0 : token - a.starts[b];
+                const int number = token - first;
                 const int place = checked_length(c, b) + number - (last ? rows_of(a, b) : 0);
                 w.position = c.seen[b] + number;
                 if (place < 0) {
@@ -92,29 +95,32 @@ __device__ __forceinline__ void find_tokens(const RowArgs& a, Where* where, bool
     __syncthreads();
 }
 
-// 8 values as they are given: 16 bytes, or 32 of fp32.
+// 8 values as they are given.
+template <int GIVEN>
 struct Given8 {
-    uint4 w[2];
+    uint4 w[GIVEN == RANS_KV_FP32 ? 2 : 1];
 };
 
-__device__ __forceinline__ void load8(Given8& x, const char* p, int given) {
+template <int GIVEN>
+__device__ __forceinline__ void load8(Given8<GIVEN>& x, const char* p) {
     x.w[0] = __ldg(reinterpret_cast<const uint4*>(p));
-    if (given == RANS_KV_FP32) x.w[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    if constexpr (GIVEN == RANS_KV_FP32) x.w[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
 }
 
-__device__ __forceinline__ void to_float(float (&x)[8], const Given8& y, int given) {
-    const uint32_t u[8] = {y.w[0].x, y.w[0].y, y.w[0].z, y.w[0].w, y.w[1].x, y.w[1].y, y.w[1].z, y.w[1].w};
-    if (given == RANS_KV_FP32) {
+template <int GIVEN>
+__device__ __forceinline__ void to_float(float (&x)[8], const Given8<GIVEN>& y) {
+    if constexpr (GIVEN == RANS_KV_FP32) {
+        x[0] = __uint_as_float(y.w[0].x); x[1] = __uint_as_float(y.w[0].y); x[2] = __uint_as_float(y.w[0].z); x[3] = __uint_as_float(y.w[0].w);
+        x[4] = __uint_as_float(y.w[1].x); x[5] = __uint_as_float(y.w[1].y); x[6] = __uint_as_float(y.w[1].z); x[7] = __uint_as_float(y.w[1].w);
+    } else {
+        const uint32_t u[4] = {y.w[0].x, y.w[0].y, y.w[0].z, y.w[0].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = given == RANS_KV_FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&u[i]))
-                                               : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = GIVEN == RANS_KV_FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&u[i]))
+                                                   : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
     }
 }
 
@@ -155,37 +161,50 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& byt
     return code;
 }
 
+template <int GIVEN>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ RowArgs a) {
     __shared__ Where where[kTokens];
+    __shared__ bool last;
     const RansKvCache& c = a.c;
-    find_tokens(a, where, false);
+    wait_for_previous();
+    let_next_start();
     const int per_row = 1 << a.part_shift, tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens);
     const int all = (tokens * c.kv_heads) << a.part_shift;
-    constexpr int kAtOnce = 2;
+    constexpr int kAtOnce = GIVEN == RANS_KV_FP32 ? 2 : 4;
+    Given8<GIVEN> in[kAtOnce][2];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
+            in[u][0] = in[u][1] = Given8<GIVEN>{};
+            if (i >= all) continue;
+            const int64_t token = blockIdx.x * kTokens + t, at = (int64_t)part * sizeof(Given8<GIVEN>);
+            load8(in[u][0], a.k_in + token * a.k_token + h * a.k_head + at);
+            load8(in[u][1], a.v_in + token * a.v_token + h * a.v_head + at);
+        }
+    };
+    load(threadIdx.x);                             // on their way while the block finds out where they go
+    find_tokens(a, where, false);
+    // The block has read its lengths; the last one to say so moves them on below.
+    int* counter = static_cast<int*>(c.workspace);
+    if (threadIdx.x == 0) {
+        last = atomicAdd(counter, 1) == (int)gridDim.x - 1;
+        if (last) *counter = 0;
+    }
     // (a row has 8 threads or more, so the four lanes of a block of 32 values are in or out of range together)
     for (int i0 = threadIdx.x; i0 - (int)(threadIdx.x & 31) < all; i0 += kThreads * kAtOnce) {
-        Given8 in[kAtOnce][2];
+        if (i0 != (int)threadIdx.x) load(i0);
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
             const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
-            if (i < all) {
-                const int64_t token = blockIdx.x * kTokens + t, at = (int64_t)part * (a.given == RANS_KV_FP32 ? 32 : 16);
-                load8(in[u][0], a.k_in + token * a.k_token + h * a.k_head + at, a.given);
-                load8(in[u][1], a.v_in + token * a.v_token + h * a.v_head + at, a.given);
-            } else {
-                in[u][0] = in[u][1] = Given8{};
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
+            if (i - (int)(threadIdx.x & 31) >= all) break;
             const Where w = where[i < all ? t : 0];
             const bool stored = i < all && w.page >= 0;
             const int64_t place = ((int64_t)w.page * c.kv_heads + h) * c.page + w.slot;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 float x[8];
-                to_float(x, in[u][v], a.given);
+                to_float(x, in[u][v]);
                 char* base = static_cast<char*>(v == 0 ? c.k : c.v);
                 const int64_t at = w.page * (v == 0 ? c.k_page : c.v_page) + h * (v == 0 ? c.k_head : c.v_head) + w.slot * (v == 0 ? c.k_slot : c.v_slot);
                 if (c.kind == RANS_KV_MXFP4) {
@@ -206,15 +225,6 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
             }
         }
     }
-    // The last block to get here (all have read the lengths by then) moves them on.
-    __shared__ bool last;
-    __syncthreads();
-    int* counter = static_cast<int*>(c.workspace);
-    if (threadIdx.x == 0) {
-        __threadfence();
-        last = atomicAdd(counter, 1) == (int)gridDim.x - 1;
-        if (last) *counter = 0;
-    }
     __syncthreads();
     if (last)
         for (int b = threadIdx.x; b < c.batch; b += kThreads) {
@@ -227,6 +237,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ RowArgs a) {
     __shared__ Where where[kTokens];
     const RansKvCache& c = a.c;
+    wait_for_previous();
+    let_next_start();
     find_tokens(a, where, true);
     const int per_row = 1 << a.part_shift, tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens);
     const int all = (tokens * c.kv_heads) << a.part_shift;
@@ -385,6 +397,8 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
     const int blocks = cluster.num_blocks(), block = cluster.block_rank(), bh = blockIdx.x / blocks;
     const int h = bh % c.kv_heads, b = bh / c.kv_heads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    wait_for_previous();
+    let_next_start();
     const int n = checked_length(c, b), k = a.budget;
     if (n > k) {
         // each block has a run of 32-place words, each warp a run of the block's
@@ -545,6 +559,8 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
 
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ EvictArgs a) {
     __shared__ int4 moving[kThreads];
+    wait_for_previous();
+    let_next_start();
     const int bh = blockIdx.y, moves = a.moves[bh];
     const int m0 = (int)((int64_t)moves * blockIdx.x / gridDim.x), m1 = (int)((int64_t)moves * (blockIdx.x + 1) / gridDim.x);
     move_rows<kThreads>(a, bh / a.c.kv_heads, bh % a.c.kv_heads, a.to + (int64_t)bh * a.budget, a.from + (int64_t)bh * a.budget, m0, m1, moving);
@@ -606,9 +622,8 @@ extern "C" int rans_kv_append(const RansKvCache* cache, const void* k, const voi
     a.k_in = static_cast<const char*>(k);
     a.v_in = static_cast<const char*>(v);
     a.k_token = k_token; a.k_head = k_head; a.v_token = v_token; a.v_head = v_head;
-    a.given = given;
-    append_kernel<<<row_grid(a), kThreads, 0, stream>>>(a);
-    return (int)cudaGetLastError();
+    auto kernel = given == RANS_KV_FP32 ? append_kernel<RANS_KV_FP32> : given == RANS_KV_FP16 ? append_kernel<RANS_KV_FP16> : append_kernel<RANS_KV_BF16>;
+    return launch_after(kernel, dim3(row_grid(a)), kThreads, 0, 1, stream, a);
 }
 
 extern "C" int rans_kv_read(const RansKvCache* cache, void* k_out, void* v_out, const int32_t* starts, int tokens,
@@ -622,8 +637,7 @@ extern "C" int rans_kv_read(const RansKvCache* cache, void* k_out, void* v_out, 
     set_rows(a, *cache, starts, tokens);
     a.k_out = static_cast<uint4*>(k_out);
     a.v_out = static_cast<uint4*>(v_out);
-    read_kernel<<<row_grid(a), kThreads, 0, stream>>>(a);
-    return (int)cudaGetLastError();
+    return launch_after(read_kernel, dim3(row_grid(a)), kThreads, 0, 1, stream, a);
 }
 
 extern "C" int64_t rans_kv_evict_bytes(const RansKvCache* c, int budget) {
@@ -661,22 +675,8 @@ extern "C" int rans_kv_evict(const RansKvCache* cache, int budget, int recent, c
         if (e != cudaSuccess) return (int)e;
         told.fetch_or(bit, std::memory_order_relaxed);
     }
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(cache->batch * cache->kv_heads * p.blocks);
-    config.blockDim = dim3(kSelect);
-    config.dynamicSmemBytes = (size_t)p.shared_keys * 4;
-    config.stream = stream;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = p.blocks;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
-    e = cudaLaunchKernelEx(&config, evict_kernel, a);
-    if (e != cudaSuccess) return (int)e;
-    if (p.apart) {
-        const int heads = cache->batch * cache->kv_heads;
-        move_kernel<<<dim3((5 * kSms + heads - 1) / heads, heads), kThreads, 0, stream>>>(a);
-    }
-    return (int)cudaGetLastError();
+    const int heads = cache->batch * cache->kv_heads;
+    const int rc2 = launch_after(evict_kernel, dim3(heads * p.blocks), kSelect, (size_t)p.shared_keys * 4, p.blocks, stream, a);
+    if (rc2 != 0 || !p.apart) return rc2;
+    return launch_after(move_kernel, dim3((4 * kSms + heads - 1) / heads, heads), kThreads, 0, 1, stream, a);
 }

@@ -49,6 +49,30 @@ __device__ __forceinline__ int checked_page(const RansKvCache& c, int b, int pag
     return p;
 }
 
+// The kernels of a step follow one another: each may start while the one before it ends, waits for it (its writes are
+// then visible) before it reads anything that changes, and lets its own follower start.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class Args>
+inline int launch_after(void (*kernel)(Args), dim3 grid, int threads, size_t shared, int cluster, cudaStream_t stream, const Args& args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args);
+    return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
 inline int64_t counter_bytes(const RansKvCache& c) {
     return 256 + (((int64_t)c.batch * c.kv_heads * kMaxSubgroups * 4 + 255) & ~(int64_t)255);
 }
