@@ -52,6 +52,9 @@ constexpr int kStart = 2;
 // 2^15, and fp16 keeps probabilities down to 2^-36 of the largest instead of 2^-25.
 constexpr float kHigh = 15.0f, kRest = 11.0f;
 
+// The maximum before there is a score: finite, so that no difference of two of them is NaN.
+constexpr float kNothing = -3.0e38f;
+
 struct AttendArgs {
     RansKvCache c;
     Divider page;
@@ -66,9 +69,10 @@ struct AttendArgs {
     int weigh;
     int* counter;                // [batch * kv_heads * subs]
     float2* stats;               // [batch * heads]: maximum (log2) and 1 / sum
-    float* part;                 // [grid][2] Attend::Part
+    float* part;                 // [grid][2] Attend::Part: what a block has of its first and last group
+    float* first;                // 4 bits: [grid][warps] Attend::Part
     float* scores;               // [tile][16][HP], scaled, log2
-    int64_t score_tiles;
+    int score_tiles;
 };
 
 __device__ __forceinline__ uint4 load16(const void* p) {
@@ -82,6 +86,9 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 __device__ __forceinline__ void copy16(void* to, const void* from, int size) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                  :: "r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -164,19 +171,22 @@ struct Attend {
         float2 ml[HP];
     };
 
-    // 4-bit tiles as they lie in the pages, copied a few tiles ahead.
-    static constexpr int kStages = 3;
+    // 4-bit tiles as they lie in the pages, copied ahead of their use; kSub of them are worked on at a time, where the
+    // registers allow two (their loop then turns half as often, and two chains of instructions run side by side).
+    static constexpr int kSub = kFp4 && NT == 1 && D <= 128 ? 2 : 1;
+    static constexpr int kStages = kSub == 2 ? 2 : 3;
     struct alignas(16) Stage {
         uint8_t k[kTile * D / 2], v[kTile * D / 2], ks[kTile * kChunks], vs[kTile * kChunks];
     };
-    // A warp's second part is written when its last tile is done, in the place of its stages.
+    // A warp's second part is written when its last tile is done, in the place of its stages.  A first part, which only a
+    // warp at a group's end has, goes to shared memory, or for 4 bits, whose stages leave no room, to the workspace.
     union Late {
         Part part;
-        Stage stage[kFp4 ? kStages : 1];
+        Stage stage[kFp4 ? kStages : 1][kSub];
     };
 
     struct Smem {
-        Part part[kWarps];                   // the warps' first parts
+        Part part[kFp4 ? 1 : kWarps];        // the warps' first parts
         Late late[kWarps];                   // their second ones
         uint4 q[kWarps][NT * kChunks * 32];  // the queries that they work on
         int tag[kWarps * 2];                 // the group of each part
@@ -290,20 +300,28 @@ struct Attend {
 
     // Starts a 4-bit tile's copy into shared memory, 16 bytes a lane; what lies behind its last token becomes zero.
     static __device__ __forceinline__ void copy_tile(Stage& st, const RansKvCache& c, const Cursor& u, int lane) {
+        constexpr int kScaleLanes = kTile * kChunks / 16;        // of the keys; as many lanes copy the values' scales
         const int at = lane * 16;
+        const bool is_k = lane < kScaleLanes;
+        const int from = at - (is_k ? 0 : kTile * kChunks);
         const uint8_t* k = static_cast<const uint8_t*>(c.k) + u.row * (D / 2) + at;
         const uint8_t* v = static_cast<const uint8_t*>(c.v) + u.row * (D / 2) + at;
+        const uint8_t* s = (is_k ? c.k_scale : c.v_scale) + u.row * kChunks + from;
+        if (u.valid == kTile) {
 #pragma unroll
-        for (int i = 0; i < kTile * D / 2; i += 512) {
-            const int size = min(max(u.valid * (D / 2) - at - i, 0), 16);
-            copy16(st.k + at + i, k + i, size);
-            copy16(st.v + at + i, v + i, size);
-        }
-        constexpr int kScaleLanes = kTile * kChunks / 16;
-        if (lane < 2 * kScaleLanes) {
-            const bool is_k = lane < kScaleLanes;
-            const int from = at - (is_k ? 0 : kTile * kChunks);
-            copy16(st.ks + at, (is_k ? c.k_scale : c.v_scale) + u.row * kChunks + from, min(max(u.valid * kChunks - from, 0), 16));
+            for (int i = 0; i < kTile * D / 2; i += 512) {
+                copy16(st.k + at + i, k + i);
+                copy16(st.v + at + i, v + i);
+            }
+            if (lane < 2 * kScaleLanes) copy16(st.ks + at, s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kTile * D / 2; i += 512) {
+                const int size = min(max(u.valid * (D / 2) - at - i, 0), 16);
+                copy16(st.k + at + i, k + i, size);
+                copy16(st.v + at + i, v + i, size);
+            }
+            if (lane < 2 * kScaleLanes) copy16(st.ks + at, s, min(max(u.valid * kChunks - from, 0), 16));
         }
     }
 
@@ -402,7 +420,7 @@ struct Attend {
             }
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) qs[(t * kChunks + j) * 32 + lane] = q[j];
-            s.m[t][0] = s.m[t][1] = -INFINITY;
+            s.m[t][0] = s.m[t][1] = kNothing;
             if constexpr (kFp4) {
 #pragma unroll
                 for (int j = 0; j < D / 64; ++j) s.unit[j] = 0;
@@ -464,35 +482,54 @@ struct Attend {
         }
     }
 
-    // The softmax's part of a tile with `valid` tokens: scores become probabilities, the maximum, the sum and O follow.
-    static __device__ __forceinline__ void probabilities(State& s, float (&sc)[NT][4], const AttendArgs& a, int64_t x, int valid,
-                                                         int lane) {
+    // The softmax's part of SUB tiles with `valid` tokens each: scores become probabilities, the maximum, the sum and O follow.
+    template <int SUB>
+    static __device__ __forceinline__ void probabilities(State& s, float (&sc)[SUB][NT][4], const AttendArgs& a, int x,
+                                                         const int (&valid)[SUB], int lane) {
         const int q4 = lane & 3, row = key_row(lane >> 2);
         bool raise_max = false;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (valid < kTile) {
-                if (row >= valid) sc[t][0] = sc[t][1] = -INFINITY;
-                if (row + 8 >= valid) sc[t][2] = sc[t][3] = -INFINITY;
+        for (int i = 0; i < SUB; ++i)
+            if (valid[i] < kTile) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (row >= valid[i]) sc[i][t][0] = sc[i][t][1] = -INFINITY;
+                    if (row + 8 >= valid[i]) sc[i][t][2] = sc[i][t][3] = -INFINITY;
+                }
             }
-            if (a.weigh && x < a.score_tiles) {
-                float* p = a.scores + (x * kTile + row) * HP + t * 8 + 2 * q4;
-                *reinterpret_cast<float2*>(p) = make_float2(sc[t][0], sc[t][1]);
-                *reinterpret_cast<float2*>(p + 8 * HP) = make_float2(sc[t][2], sc[t][3]);
+        if (a.weigh) {
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) {
+                if (valid[i] == 0 || x + i >= a.score_tiles) continue;
+                float* p = a.scores + ((int64_t)(x + i) * kTile + row) * HP + 2 * q4;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    *reinterpret_cast<float2*>(p + t * 8) = make_float2(sc[i][t][0], sc[i][t][1]);
+                    *reinterpret_cast<float2*>(p + t * 8 + 8 * HP) = make_float2(sc[i][t][2], sc[i][t][3]);
+                }
             }
-            raise_max |= fmaxf(sc[t][0], sc[t][2]) > s.m[t][0] + kHigh || fmaxf(sc[t][1], sc[t][3]) > s.m[t][1] + kHigh;
         }
+        float top[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                top[t][e] = fmaxf(sc[0][t][e], sc[0][t][e + 2]);
+#pragma unroll
+                for (int i = 1; i < SUB; ++i) top[t][e] = fmaxf(top[t][e], fmaxf(sc[i][t][e], sc[i][t][e + 2]));
+                raise_max |= top[t][e] > s.m[t][e] + kHigh;
+            }
         if (__any_sync(~0u, raise_max)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float m = fmaxf(sc[t][e], sc[t][e + 2]);
+                    float m = top[t][e];
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
                     m = fmaxf(m - kRest, s.m[t][e]);
-                    const float f = m == -INFINITY ? 1.0f : exp2_fast(s.m[t][e] - m);
+                    const float f = exp2_fast(s.m[t][e] - m);
                     s.m[t][e] = m;
                     s.l[t][e] *= f;
 #pragma unroll
@@ -503,15 +540,14 @@ struct Attend {
                 }
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float m0 = s.m[t][0] == -INFINITY ? 0.0f : s.m[t][0], m1 = s.m[t][1] == -INFINITY ? 0.0f : s.m[t][1];
-            sc[t][0] = exp2_fast(sc[t][0] - m0);
-            sc[t][1] = exp2_fast(sc[t][1] - m1);
-            sc[t][2] = exp2_fast(sc[t][2] - m0);
-            sc[t][3] = exp2_fast(sc[t][3] - m1);
-            s.l[t][0] += sc[t][0] + sc[t][2];
-            s.l[t][1] += sc[t][1] + sc[t][3];
-        }
+        for (int i = 0; i < SUB; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[i][t][e] = exp2_fast(sc[i][t][e] - s.m[t][e & 1]);
+                s.l[t][0] += sc[i][t][0] + sc[i][t][2];
+                s.l[t][1] += sc[i][t][1] + sc[i][t][3];
+            }
     }
 
     // P^T's operands from a tile's probabilities.
@@ -544,8 +580,9 @@ struct Attend {
         }
     }
 
-    // fp16 factors 2^(scale byte - unit) of a lane's words, for bytes from unit - 7 to unit + 8; whether some tile's are outside.
-    static __device__ __forceinline__ bool factors(uint32_t (&f)[D / 64][2], const State& s, const CodeV& r) {
+    // fp16 factors 2^(scale byte - unit) of a lane's words, for bytes from unit - 7 to unit + 8; nonzero bits under 0xfff0fff0
+    // where some are outside.
+    static __device__ __forceinline__ uint32_t factors(uint32_t (&f)[D / 64][2], const State& s, const CodeV& r) {
         uint32_t outside = 0;
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
@@ -560,40 +597,73 @@ struct Attend {
                 f[j][k] = in * 1024u + 0x20002000u;
             }
         }
-        return __any_sync(~0u, (outside & 0xfff0fff0u) != 0);
+        return outside;
     }
 
-    static __device__ __forceinline__ void accumulate(State& s, const CodeV& r, const float (&p)[NT][4]) {
-        uint32_t f[D / 64][2];
-        bool wide = factors(f, s, r);
-        if (wide) {
-            raise_unit(s, r);
-            wide = factors(f, s, r);
+    // Rows behind a tile's last token hold zeros, their scale bytes too: these become the units, so that a group's last tile
+    // is like any other.
+    static __device__ __forceinline__ void fill_scales(CodeV& r, const State& s, int valid, int q4) {
+        uint32_t units = 0;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) units |= (uint32_t)s.unit[j] << (8 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (value_row(q4, i) >= valid) r.s[i] = units;
+    }
+
+    // O^T += V^T P^T over the first `count` of kSub tiles.
+    static __device__ __forceinline__ void accumulate(State& s, CodeV (&r)[kSub], const float (&p)[kSub][NT][4],
+                                                      const int (&valid)[kSub], int count, int lane) {
+        uint32_t f[kSub][D / 64][2];
+        auto wide = [&]() {
+#pragma unroll
+            for (int i = 0; i < kSub; ++i)
+                if (valid[i] < kTile) fill_scales(r[i], s, valid[i], lane & 3);
+            uint32_t outside = factors(f[0], s, r[0]);
+#pragma unroll
+            for (int i = 1; i < kSub; ++i) {
+                const uint32_t more = factors(f[i], s, r[i]);
+                if (i < count) outside |= more;
+            }
+            return __any_sync(~0u, (outside & 0xfff0fff0u) != 0);
+        };
+        bool any_wide = wide();
+        if (any_wide) {
+#pragma unroll
+            for (int i = 0; i < kSub; ++i)
+                if (i < count) raise_unit(s, r[i]);
+            any_wide = wide();
         }
-        if (wide) {
-            accumulate_wide(s, r, p);
+        if (any_wide) {
+#pragma unroll
+            for (int i = 0; i < kSub; ++i)
+                if (i < count) accumulate_wide(s, r[i], p[i]);
             return;
         }
-        uint32_t pb[NT][2];
-        pack_probabilities<true>(pb, p);
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-            // two tokens' codes of one column next to each other: columns 0, 2, 4, 6 and 1, 3, 5, 7
-            const uint32_t even0 = (r.w[0][j] & 0x0f0f0f0fu) | ((r.w[1][j] << 4) & 0xf0f0f0f0u);
-            const uint32_t odd0 = ((r.w[0][j] >> 4) & 0x0f0f0f0fu) | (r.w[1][j] & 0xf0f0f0f0u);
-            const uint32_t even1 = (r.w[2][j] & 0x0f0f0f0fu) | ((r.w[3][j] << 4) & 0xf0f0f0f0u);
-            const uint32_t odd1 = ((r.w[2][j] >> 4) & 0x0f0f0f0fu) | (r.w[3][j] & 0xf0f0f0f0u);
-            uint32_t e0[4], o0[4], e1[4], o1[4];
-            e2m1_to_half(e0, even0);
-            e2m1_to_half(o0, odd0);
-            e2m1_to_half(e1, even1);
-            e2m1_to_half(o1, odd1);
+        for (int i = 0; i < kSub; ++i) {
+            if (i >= count) break;
+            uint32_t pb[NT][2];
+            pack_probabilities<true>(pb, p[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a0 = multiply2(e0[i], f[j][0]), a1 = multiply2(o0[i], f[j][0]);
-                const uint32_t a2 = multiply2(e1[i], f[j][1]), a3 = multiply2(o1[i], f[j][1]);
+            for (int j = 0; j < D / 64; ++j) {
+                // two tokens' codes of one column next to each other: columns 0, 2, 4, 6 and 1, 3, 5, 7
+                const uint32_t even0 = (r[i].w[0][j] & 0x0f0f0f0fu) | ((r[i].w[1][j] << 4) & 0xf0f0f0f0u);
+                const uint32_t odd0 = ((r[i].w[0][j] >> 4) & 0x0f0f0f0fu) | (r[i].w[1][j] & 0xf0f0f0f0u);
+                const uint32_t even1 = (r[i].w[2][j] & 0x0f0f0f0fu) | ((r[i].w[3][j] << 4) & 0xf0f0f0f0u);
+                const uint32_t odd1 = ((r[i].w[2][j] >> 4) & 0x0f0f0f0fu) | (r[i].w[3][j] & 0xf0f0f0f0u);
+                uint32_t e0[4], o0[4], e1[4], o1[4];
+                e2m1_to_half(e0, even0);
+                e2m1_to_half(o0, odd0);
+                e2m1_to_half(e1, even1);
+                e2m1_to_half(o1, odd1);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma<true>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t a0 = multiply2(e0[d], f[i][j][0]), a1 = multiply2(o0[d], f[i][j][0]);
+                    const uint32_t a2 = multiply2(e1[d], f[i][j][1]), a3 = multiply2(o1[d], f[i][j][1]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) mma<true>(s.o[j * 4 + d][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                }
             }
         }
     }
@@ -863,6 +933,10 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     auto heads_of = [&](const Group& s) { return min(a.sub_heads, a.group - s.sub * a.sub_heads); };
     auto head0_of = [&](const Group& s) { return s.h * a.group + s.sub * a.sub_heads; };
 
+    auto first_part = [&](int w) {
+        if constexpr (A::kFp4) return reinterpret_cast<typename A::Part*>(a.first) + blockIdx.x * W + w;
+        else return &sm.part[w];
+    };
     Group s{};
     int nt = 0, tile = 0;
     auto next_group = [&](Group& s, int& nt, int& tile) {
@@ -903,31 +977,35 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             if (whole && ends) {
                 A::write_out(st, a, of.b, head0_of(of), heads_of(of), lane);
             } else {
-                A::write_part(st, flushed == 0 ? sm.part[warp] : sm.late[warp].part, lane);
+                A::write_part(st, flushed == 0 ? *first_part(warp) : sm.late[warp].part, lane);
                 if (lane == 0) sm.tag[flushed * W + warp] = of.pack();
                 ++flushed;
             }
         };
         if constexpr (A::kFp4) {
-            // The copies run kStages - 1 tiles ahead, in places of their own (`ahead`).
-            constexpr int kStages = A::kStages;
-            typename A::Stage* stages = sm.late[warp].stage;
+            // The copies run kStages - 1 turns ahead, in places of their own (`ahead`).  A turn takes kSub tiles of a group, or
+            // what is left of it.
+            constexpr int kStages = A::kStages, kSub = A::kSub;
+            auto stages = sm.late[warp].stage;
             Group ahead = s;
             int ahead_nt = nt, ahead_tile = tile, ahead_x = x;
-            uint32_t valid = 0;                          // of each stage, 8 bits
+            uint32_t valid = 0;                          // tokens of each stage's tiles, 5 bits each
             bool fresh = true, ahead_fresh = true;
             auto copy = [&](int stage) {
-                if (ahead_x < xe) {
+#pragma unroll
+                for (int i = 0; i < kSub; ++i) {
+                    if (ahead_x >= xe || (i > 0 && ahead_fresh)) break;
                     if (ahead_fresh) u.begin(c, a.page, ahead.b, ahead.h, checked_length(c, ahead.b), ahead_tile, lane);
                     else u.advance(c, ahead.b, ahead.h, lane);
-                    valid = (valid & ~(255u << (8 * stage))) | (uint32_t)u.valid << (8 * stage);
-                    A::copy_tile(stages[stage], c, u, lane);
+                    const int at = (stage * kSub + i) * 5;
+                    valid = (valid & ~(31u << at)) | (uint32_t)u.valid << at;
+                    A::copy_tile(stages[stage][i], c, u, lane);
                     ++ahead_x;
                     ahead_fresh = ++ahead_tile == ahead_nt;
-                    if (ahead_fresh) {
-                        ahead_x += kStart;
-                        if (ahead_x < xe) next_group(ahead, ahead_nt, ahead_tile);
-                    }
+                }
+                if (ahead_fresh && ahead_tile == ahead_nt) {
+                    ahead_x += kStart;
+                    if (ahead_x < xe) next_group(ahead, ahead_nt, ahead_tile); else ahead_tile = 0;
                 }
                 copies_end();
             };
@@ -937,18 +1015,26 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             for (int stage = 0, free = kStages - 1;; free = stage, stage = stage == kStages - 1 ? 0 : stage + 1) {
                 if (fresh) A::begin(st, qs, a, s.b, head0_of(s), heads_of(s), lane);
                 copies_wait<kStages - 2>();
-                __syncwarp();                            // all lanes' copies of this tile are there, and the tile before it is read
+                __syncwarp();                            // all lanes' copies of these tiles are there, and those before are read
                 copy(free);
-                float sc[NT][4];
-                typename A::CodeK ck;
-                A::read_k(ck, stages[stage], lane);
-                A::scores(st, qs, ck, a, sc, lane);
-                A::probabilities(st, sc, a, x, (int)(valid >> (8 * stage)) & 255, lane);
-                typename A::CodeV cv;
-                A::read_v(cv, stages[stage], lane);
-                A::accumulate(st, cv, sc);
-                fresh = ++tile == nt;
-                x += 1 + (fresh ? kStart : 0);
+                const int count = kSub == 1 ? 1 : min(min(kSub, nt - tile), xe - x);
+                float sc[kSub][NT][4];
+                int tokens[kSub];
+#pragma unroll
+                for (int i = 0; i < kSub; ++i) {
+                    tokens[i] = i < count ? (int)(valid >> ((stage * kSub + i) * 5)) & 31 : 0;
+                    typename A::CodeK ck;
+                    A::read_k(ck, stages[stage][i], lane);   // (of a missing tile: whatever is there, masked below)
+                    A::scores(st, qs, ck, a, sc[i], lane);
+                }
+                A::probabilities(st, sc, a, x, tokens, lane);
+                typename A::CodeV cv[kSub];
+#pragma unroll
+                for (int i = 0; i < kSub; ++i) A::read_v(cv[i], stages[stage][i], lane);
+                A::accumulate(st, cv, sc, tokens, count, lane);
+                tile += count;
+                fresh = tile == nt;
+                x += count + (fresh ? kStart : 0);
                 if (fresh || x >= xe) flush(s, fresh);
                 if (x >= xe) break;
                 if (fresh) {
@@ -964,16 +1050,16 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             bool have = false, fresh = true;
 #pragma unroll 1
             while (true) {
-                float sc[NT][4];
+                float sc[1][NT][4];
                 bool more = true, ends = false;
                 const Group now = s;
-                int next = x, valid = 0;
+                int next = x, valid[1] = {0};
                 if (have) {
-                    A::scores(st, qs, rk, a, sc, lane);
+                    A::scores(st, qs, rk, a, sc[0], lane);
                     ends = ++tile == nt;
                     next = x + 1 + (ends ? kStart : 0);
                     more = next < xe;
-                    valid = u.valid;
+                    valid[0] = u.valid;
                     fresh = ends;
                     if (ends && more) next_group(s, nt, tile);
                 }
@@ -983,7 +1069,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                 }
                 if (have) {
                     A::probabilities(st, sc, a, x, valid, lane);
-                    A::accumulate(st, rv, sc);
+                    A::accumulate(st, rv, sc[0]);
                     x = next;
                     if (ends || !more) flush(now, ends);
                 }
@@ -1000,13 +1086,15 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
     }
     __syncthreads();
 
-    // Join the warps' parts group by group (each warp finds the groups for itself); what the block has not all of goes to
-    // the workspace.
+    // Join the warps' parts group by group; what the block has not all of goes to the workspace.  Each warp finds the groups
+    // for itself, and the warps take turns at 32 columns of a group.
     static_assert(W * 2 <= 32, "one lane per part");
     constexpr int kVec = HP * (D / 4);
     typename A::Part* parts = reinterpret_cast<typename A::Part*>(a.part);
     int open0 = -1, open1 = -1;                          // groups that the block has only some of: its first, its last
     const int my_tag = lane < W * 2 ? sm.tag[lane] : -1;
+    constexpr int kSlices = kVec / 32;
+    int turn = warp;                                     // of this group's slices: turn, turn + W, ..
     for (unsigned left = __ballot_sync(~0u, my_tag >= 0); left != 0;) {
         const int tag = __shfl_sync(~0u, my_tag, __ffs(left) - 1);
         const unsigned run = __ballot_sync(~0u, my_tag == tag);
@@ -1024,13 +1112,13 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                 if (f0 < start + nt && start + nt <= f1) sm.last_block[slot] = tid;
             }
         }
-        for (int v = tid; v < kVec; v += kThreads) {
-            const int head = v / (D / 4), d = v % (D / 4) * 4;
-            if (head >= heads) break;
+        for (; turn < kSlices; turn += W) {
+            const int v = turn * 32 + lane, head = v / (D / 4), d = v % (D / 4) * 4;
+            if (head >= heads) continue;
             float4 o;
             float top, l;
             unsigned rest = run;
-            A::template join<true>([&](int) { const int e = __ffs(rest) - 1; rest &= rest - 1; return e < W ? &sm.part[e] : &sm.late[e - W].part; }, __popc(run), head, d, o, top, l);
+            A::template join<true>([&](int) { const int e = __ffs(rest) - 1; rest &= rest - 1; return e < W ? (const typename A::Part*)first_part(e) : &sm.late[e - W].part; }, __popc(run), head, d, o, top, l);
             if (whole) {
                 A::store_joined(a, s.b, head0_of(s) + head, d, o, top, l);
             } else {
@@ -1039,6 +1127,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                 if (d == 0) __stcg(&mine->ml[head], make_float2(top, l));
             }
         }
+        turn -= kSlices;
     }
 
     // The last block of a group to get here joins the blocks' parts.
@@ -1174,7 +1263,7 @@ __global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_const
 
 struct Plan {
     int nt, subs, sub_heads;
-    int64_t counter, stats, part, scores, bytes, score_tiles;
+    int64_t counter, stats, part, first, scores, bytes, score_tiles;
 };
 
 bool make_plan(const RansKvCache& c, int heads, int weigh, Plan& p) {
@@ -1190,9 +1279,12 @@ bool make_plan(const RansKvCache& c, int heads, int weigh, Plan& p) {
     p.counter = 256;
     p.stats = counter_bytes(c);
     p.part = p.stats + up((int64_t)c.batch * heads * 8);
-    p.scores = p.part + up((int64_t)kGrid * 2 * p.nt * 8 * (c.dim + 4 + 2) * 4);
+    const int64_t part = (int64_t)p.nt * 8 * (c.dim + 4 + 2) * 4;            // sizeof(Attend::Part)
+    p.first = p.part + up(kGrid * 2 * part);
+    p.scores = p.first + (c.kind == RANS_KV_MXFP4 ? up(kGrid * 16 * part) : 0);
     // every token of every page, and the places behind the groups' last tiles
     p.score_tiles = weigh ? ((int64_t)c.pages * c.page / kTile + (int64_t)c.batch * kStart) * c.kv_heads * p.subs : 0;
+    if (p.score_tiles > 0x7fffffff) return false;
     p.bytes = p.scores + up(p.score_tiles * kTile * p.nt * 8 * 4);
     return true;
 }
@@ -1273,7 +1365,8 @@ extern "C" int rans_kv_attend(const RansKvCache* cache, const void* q, int q_kin
     a.stats = reinterpret_cast<float2*>(ws + p.stats);
     a.part = reinterpret_cast<float*>(ws + p.part);
     a.scores = reinterpret_cast<float*>(ws + p.scores);
-    a.score_tiles = p.score_tiles;
+    a.first = reinterpret_cast<float*>(ws + p.first);
+    a.score_tiles = (int)p.score_tiles;
     int e;
     switch (cache->kind) {
         case RANS_KV_BF16: e = launch_kind<RANS_KV_BF16>(a, p.nt, stream); break;
