@@ -352,6 +352,20 @@ def test_evict(torch, rc, weights, budget, recent):
     _evict_case(torch, rc, [0, 1, budget, budget + 1, 300], 2, 64, 16, "bf16", SOME[weights], budget, recent, seed=budget)
 
 
+@pytest.mark.parametrize("weights", list(SOME))
+@pytest.mark.parametrize("budget,recent", [(1, 1), (5, 0), (64, 60), (200, 3)])
+def test_evict_a_few(torch, rc, weights, budget, recent):
+    """One to five tokens over the budget: the search one by one and the first one beyond it."""
+    _evict_case(torch, rc, [budget + i for i in range(1, 6)], 2, 64, 16, "bf16", SOME[weights], budget, recent, seed=budget)
+
+
+@pytest.mark.parametrize("over", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("weights", ["random", "equal", "few values"])
+def test_evict_a_few_of_many(torch, rc, over, weights):
+    """The same with several blocks to a head."""
+    _evict_case(torch, rc, [30000 + over], 1, 64, 64, "fp16", SOME[weights], 30000, 100, seed=over)
+
+
 @pytest.mark.parametrize("kind,dim,page", [("fp16", 128, 32), ("mxfp4", 64, 16), ("mxfp4", 128, 48), ("mxfp4", 256, 16), ("bf16", 256, 64)])
 def test_evict_kinds(torch, rc, kind, dim, page):
     _evict_case(torch, rc, [200, 90, 33], 3, dim, page, kind, SOME["random"], 60, 16)

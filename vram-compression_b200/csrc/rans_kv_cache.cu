@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 constexpr int kSelect = 1024;
 constexpr int kSelectWarps = kSelect / 32;
 constexpr int kBins = 2048;                                // two per thread
+constexpr int kFew = 4;                                    // tokens over the budget that are searched for one by one
 constexpr int kMaxCluster = 8;                             // the portable size; of 16, seven at most run at a time
 constexpr int kPlaces = 4096;                              // a block takes before there are more of them
 constexpr int kMaxSharedKeys = 40 * 1024;                  // of a block; more are kept in the workspace
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
     extern __shared__ uint32_t shared_keys[];
     __shared__ __align__(8) int hist[2][kBins];
     __shared__ int digit_s, rank_s, count_s;
+    __shared__ uint2 lightest[kFew];                       // the block's lightest token of each turn: key, place
     __shared__ int wsum[2][kSelectWarps];
     __shared__ int block_sum[3];                           // ties, holes, movers of the block's places
     __shared__ int4 moving[kSelect];                       // (page, slot) to and from
@@ -426,117 +428,181 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
             for (int i = 0; i < kLoads; ++i)
                 if (t0 + i * kSelect < t_end) keys[t0 + i * kSelect] = at[i] >= 0 ? key_of(weight[i], position[i] >= first_late) : 0;
         }
-        uint32_t prefix = 0;
-        int rank = k;                                      // of the threshold among the keys that share the prefix
         auto sync = [&]() {
             if (blocks == 1) __syncthreads(); else cluster.sync();
         };
+        int *to = a.to + (int64_t)bh * k, *from = a.from + (int64_t)bh * k;
+        int moves = 0;
+        if (n - k <= kFew) {
+            // A few too many, as in a loop that evicts as it appends: the lightest (of equals the last) goes, n - k times.
+            int gone[kFew];
+#pragma unroll
+            for (int turn = 0; turn < kFew; ++turn) {
+                gone[turn] = -1;
+                if (turn >= n - k) continue;
+                __syncthreads();
+                uint32_t key = 0xffffffffu;
+                int place = -1;
+                for (int t = w0 * 32 + lane; t < min(w1 * 32, n); t += 32) {
+                    bool out = false;
+#pragma unroll
+                    for (int i = 0; i < turn; ++i) out |= t == gone[i];
+                    if (!out && keys[t] <= key) {
+                        key = keys[t];
+                        place = t;
+                    }
+                }
+                uint32_t least = __reduce_min_sync(~0u, key);
+                int last = __reduce_max_sync(~0u, key == least ? place : -1);
+                if (lane == 0) {
+                    wsum[0][warp] = (int)least;
+                    wsum[1][warp] = last;
+                }
+                __syncthreads();
+                key = (uint32_t)wsum[0][lane];
+                place = wsum[1][lane];
+                least = __reduce_min_sync(~0u, place >= 0 ? key : 0xffffffffu);
+                last = __reduce_max_sync(~0u, key == least ? place : -1);
+                if (blocks > 1) {
+                    if (tid == 0) lightest[turn] = make_uint2(least, (uint32_t)last);
+                    cluster.sync();
+                    const uint2 x = lane < blocks ? *cluster.map_shared_rank(&lightest[turn], lane) : make_uint2(0xffffffffu, (uint32_t)-1);
+                    least = __reduce_min_sync(~0u, (int)x.y >= 0 ? x.x : 0xffffffffu);
+                    last = __reduce_max_sync(~0u, x.x == least ? (int)x.y : -1);
+                }
+                gone[turn] = last;
+            }
+            if (block == 0 && tid == 0) {
+                // the freed places below the budget, rising, and the kept ones above it
+                int holes = 0, kept = 0;
+                for (int above = -1;;) {
+                    int next = k;
+#pragma unroll
+                    for (int i = 0; i < kFew; ++i)
+                        if (gone[i] > above && gone[i] < next) next = gone[i];
+                    if (next == k) break;
+                    to[holes++] = above = next;
+                }
+                for (int t = k; t < n; ++t) {
+                    bool out = false;
+#pragma unroll
+                    for (int i = 0; i < kFew; ++i) out |= t == gone[i];
+                    if (!out) from[kept++] = t;
+                }
+                block_sum[1] = holes;
+            }
+            sync();
+            moves = *cluster.map_shared_rank(&block_sum[1], 0);
+            if (blocks > 1) cluster.sync();                // block 0 stays until all have read
+        } else {
+            uint32_t prefix = 0;
+            int rank = k;                                      // of the threshold among the keys that share the prefix
 #pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            const uint32_t mask = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;        // of the digits found
-            int* mine = hist[pass & 1];
-            mine[tid] = mine[tid + kSelect] = 0;
-            __syncthreads();
-            for (int w = w0; w < w1; ++w) {
+            for (int pass = 0; pass < 3; ++pass) {
+                const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+                const uint32_t mask = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;        // of the digits found
+                int* mine = hist[pass & 1];
+                mine[tid] = mine[tid + kSelect] = 0;
+                __syncthreads();
+                for (int w = w0; w < w1; ++w) {
+                    const int t = w * 32 + lane;
+                    const uint32_t key = t < n ? keys[t] : 0;
+                    if (t < n && (key & mask) == prefix) atomicAdd(&mine[(key >> shift) & (kBins - 1)], 1);
+                }
+                sync();
+                // thread i: the bins kBins - 1 - 2 i and the one below, of all blocks
+                int2 sum = make_int2(0, 0);
+                for (int r = 0; r < blocks; ++r) {
+                    const int2 x = reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r))[kSelect - 1 - tid];
+                    sum.x += x.y;
+                    sum.y += x.x;
+                }
+                int inc = sum.x + sum.y;
+#pragma unroll
+                for (int i = 1; i < 32; i *= 2) {
+                    const int y = __shfl_up_sync(~0u, inc, i);
+                    if (lane >= i) inc += y;
+                }
+                if (lane == 31) wsum[pass & 1][warp] = inc;
+                __syncthreads();
+                const int before = inc - sum.x - sum.y + warp_sum(lane < warp ? wsum[pass & 1][lane] : 0);
+                if (before < rank && rank <= before + sum.x + sum.y) {
+                    const bool second = rank > before + sum.x;
+                    digit_s = kBins - 1 - 2 * tid - (second ? 1 : 0);
+                    rank_s = rank - before - (second ? sum.x : 0);
+                    count_s = second ? sum.y : sum.x;
+                }
+                __syncthreads();
+                prefix |= (uint32_t)digit_s << shift;
+                rank = rank_s;
+                if (rank == count_s) {
+                    // all that share these digits stay: no ties to part.  (prefix > 0, for n > budget keys are not all kept.)
+                    --prefix;
+                    rank = 0;
+                    break;
+                }
+            }
+            // Keys above `prefix` stay, and the first `rank` places whose key equals it.
+            int tie0 = 0;
+            if (rank > 0) {
+                int ties = 0;
+                for (int w = w0; w < w1; ++w) {
+                    const int t = w * 32 + lane;
+                    ties += __popc(__ballot_sync(~0u, t < n && keys[t] == prefix));
+                }
+                __syncthreads();
+                if (lane == 0) wsum[0][warp] = ties;
+                __syncthreads();
+                tie0 = warp_sum(lane < warp ? wsum[0][lane] : 0);
+                if (tid == kSelect - 1) block_sum[0] = tie0 + ties;
+                sync();
+                tie0 += warp_sum(lane < block ? *cluster.map_shared_rank(&block_sum[0], lane) : 0);
+            }
+            auto kept = [&](int w, int& tie) {
                 const int t = w * 32 + lane;
                 const uint32_t key = t < n ? keys[t] : 0;
-                if (t < n && (key & mask) == prefix) atomicAdd(&mine[(key >> shift) & (kBins - 1)], 1);
-            }
-            sync();
-            // thread i: the bins kBins - 1 - 2 i and the one below, of all blocks
-            int2 sum = make_int2(0, 0);
-            for (int r = 0; r < blocks; ++r) {
-                const int2 x = reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r))[kSelect - 1 - tid];
-                sum.x += x.y;
-                sum.y += x.x;
-            }
-            int inc = sum.x + sum.y;
-#pragma unroll
-            for (int i = 1; i < 32; i *= 2) {
-                const int y = __shfl_up_sync(~0u, inc, i);
-                if (lane >= i) inc += y;
-            }
-            if (lane == 31) wsum[pass & 1][warp] = inc;
-            __syncthreads();
-            const int before = inc - sum.x - sum.y + warp_sum(lane < warp ? wsum[pass & 1][lane] : 0);
-            if (before < rank && rank <= before + sum.x + sum.y) {
-                const bool second = rank > before + sum.x;
-                digit_s = kBins - 1 - 2 * tid - (second ? 1 : 0);
-                rank_s = rank - before - (second ? sum.x : 0);
-                count_s = second ? sum.y : sum.x;
-            }
-            __syncthreads();
-            prefix |= (uint32_t)digit_s << shift;
-            rank = rank_s;
-            if (rank == count_s) {
-                // all that share these digits stay: no ties to part.  (prefix > 0, for n > budget keys are not all kept.)
-                --prefix;
-                rank = 0;
-                break;
-            }
-        }
-        // Keys above `prefix` stay, and the first `rank` places whose key equals it.
-        int tie0 = 0;
-        if (rank > 0) {
-            int ties = 0;
+                const unsigned equal = __ballot_sync(~0u, t < n && key == prefix);
+                const bool keep = t < n && (key > prefix || (key == prefix && tie + __popc(equal & ((1u << lane) - 1)) < rank));
+                tie += __popc(equal);
+                return keep;
+            };
+            int holes = 0, movers = 0, tie = tie0;
             for (int w = w0; w < w1; ++w) {
                 const int t = w * 32 + lane;
-                ties += __popc(__ballot_sync(~0u, t < n && keys[t] == prefix));
+                const bool keep = kept(w, tie);
+                holes += __popc(__ballot_sync(~0u, t < k && !keep));
+                movers += __popc(__ballot_sync(~0u, t >= k && keep));
             }
             __syncthreads();
-            if (lane == 0) wsum[0][warp] = ties;
+            if (lane == 0) {
+                wsum[0][warp] = holes;
+                wsum[1][warp] = movers;
+            }
             __syncthreads();
-            tie0 = warp_sum(lane < warp ? wsum[0][lane] : 0);
-            if (tid == kSelect - 1) block_sum[0] = tie0 + ties;
+            int hole = warp_sum(lane < warp ? wsum[0][lane] : 0), mover = warp_sum(lane < warp ? wsum[1][lane] : 0);
+            if (tid == kSelect - 1) {
+                block_sum[1] = hole + holes;
+                block_sum[2] = mover + movers;
+            }
             sync();
-            tie0 += warp_sum(lane < block ? *cluster.map_shared_rank(&block_sum[0], lane) : 0);
+            const int block_holes = lane < blocks ? *cluster.map_shared_rank(&block_sum[1], lane) : 0;
+            const int block_movers = lane < blocks ? *cluster.map_shared_rank(&block_sum[2], lane) : 0;
+            hole += warp_sum(lane < block ? block_holes : 0);
+            mover += warp_sum(lane < block ? block_movers : 0);
+            moves = warp_sum(block_holes);
+            tie = tie0;
+            for (int w = w0; w < w1; ++w) {
+                const int t = w * 32 + lane;
+                const bool keep = kept(w, tie);
+                const unsigned is_hole = __ballot_sync(~0u, t < k && !keep), is_mover = __ballot_sync(~0u, t >= k && keep);
+                const unsigned below = (1u << lane) - 1;
+                if (is_hole >> lane & 1) to[hole + __popc(is_hole & below)] = t;
+                if (is_mover >> lane & 1) from[mover + __popc(is_mover & below)] = t;
+                hole += __popc(is_hole);
+                mover += __popc(is_mover);
+            }
+            sync();                                            // the lists are whole; nobody reads another block's memory from here on
         }
-        auto kept = [&](int w, int& tie) {
-            const int t = w * 32 + lane;
-            const uint32_t key = t < n ? keys[t] : 0;
-            const unsigned equal = __ballot_sync(~0u, t < n && key == prefix);
-            const bool keep = t < n && (key > prefix || (key == prefix && tie + __popc(equal & ((1u << lane) - 1)) < rank));
-            tie += __popc(equal);
-            return keep;
-        };
-        int holes = 0, movers = 0, tie = tie0;
-        for (int w = w0; w < w1; ++w) {
-            const int t = w * 32 + lane;
-            const bool keep = kept(w, tie);
-            holes += __popc(__ballot_sync(~0u, t < k && !keep));
-            movers += __popc(__ballot_sync(~0u, t >= k && keep));
-        }
-        __syncthreads();
-        if (lane == 0) {
-            wsum[0][warp] = holes;
-            wsum[1][warp] = movers;
-        }
-        __syncthreads();
-        int hole = warp_sum(lane < warp ? wsum[0][lane] : 0), mover = warp_sum(lane < warp ? wsum[1][lane] : 0);
-        if (tid == kSelect - 1) {
-            block_sum[1] = hole + holes;
-            block_sum[2] = mover + movers;
-        }
-        sync();
-        const int block_holes = lane < blocks ? *cluster.map_shared_rank(&block_sum[1], lane) : 0;
-        const int block_movers = lane < blocks ? *cluster.map_shared_rank(&block_sum[2], lane) : 0;
-        hole += warp_sum(lane < block ? block_holes : 0);
-        mover += warp_sum(lane < block ? block_movers : 0);
-        const int moves = warp_sum(block_holes);
-        int *to = a.to + (int64_t)bh * k, *from = a.from + (int64_t)bh * k;
-        tie = tie0;
-        for (int w = w0; w < w1; ++w) {
-            const int t = w * 32 + lane;
-            const bool keep = kept(w, tie);
-            const unsigned is_hole = __ballot_sync(~0u, t < k && !keep), is_mover = __ballot_sync(~0u, t >= k && keep);
-            const unsigned below = (1u << lane) - 1;
-            if (is_hole >> lane & 1) to[hole + __popc(is_hole & below)] = t;
-            if (is_mover >> lane & 1) from[mover + __popc(is_mover & below)] = t;
-            hole += __popc(is_hole);
-            mover += __popc(is_mover);
-        }
-        sync();                                            // the lists are whole; nobody reads another block's memory from here on
 
         if (a.moves != nullptr) {
             if (block == 0 && tid == 0) a.moves[bh] = moves;
