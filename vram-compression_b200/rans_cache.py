@@ -167,7 +167,7 @@ class KVCache:
         return self._raw_stream(self._index)
 
     def _rows(self, k, v):
-        """Checks of append's rows, which depend on their shapes alone: (type, bytes a value, strides are usable)."""
+        """Checks of append's rows, which depend on their shapes alone: (type, strides are usable, strides in bytes)."""
         torch = self._torch
         for x, what in ((k, "k"), (v, "v")):
             _need(x.device == self.device and x.dim() == 3 and tuple(x.shape[1:]) == (self.kv_heads, self.dim),
@@ -177,21 +177,23 @@ class KVCache:
         _need(given is not None, "k and v must be bf16, fp16 or fp32")
         size = k.element_size()
         usable = lambda x: x.stride(2) == 1 and x.stride(0) * size % 16 == 0 and x.stride(1) * size % 16 == 0   # noqa: E731
-        return given, size, usable(k), usable(v)
+        return given, usable(k), usable(v), *(x.stride(i) * size for x in (k, v) for i in range(2))
 
     @staticmethod
     def _aligned(x, usable):
-        """x itself, or a copy whose rows can be read 16 bytes at a time."""
+        """x itself, or a contiguous copy, so that rows can be read 16 bytes at a time."""
         if usable and x.data_ptr() % 16 == 0:
             return x
         return x.clone() if x.is_contiguous() else x.contiguous()
 
     def _starts(self, starts, tokens):
         if starts is None:
-            _need(tokens == self.batch, f"without starts there is one token for each of the {self.batch} sequences")
+            if tokens != self.batch:
+                raise ValueError(f"without starts there is one token for each of the {self.batch} sequences")
             return None
-        _need(starts.dtype == self._torch.int32 and starts.get_device() == self._index and starts.numel() == self.batch + 1
-              and starts.is_contiguous(), f"starts must be contiguous int32 [{self.batch + 1}] on {self.device}")
+        if (starts.dtype != self._torch.int32 or starts.get_device() != self._index or starts.numel() != self.batch + 1
+                or not starts.is_contiguous()):
+            raise ValueError(f"starts must be contiguous int32 [{self.batch + 1}] on {self.device}")
         return starts.data_ptr()
 
     # ---------------------------------------------------------------- pages
@@ -239,13 +241,16 @@ class KVCache:
         known = self._sizes.get(key)
         if known is None:
             known = self._sizes[key] = self._rows(k, v)
-        given, size, k_usable, v_usable = known
-        _need(k.get_device() == self._index and v.get_device() == self._index, f"k and v must be on {self.device}")
-        k, v, n = self._aligned(k, k_usable), self._aligned(v, v_usable), k.shape[0]
-        kt, kh, _ = k.stride()
-        vt, vh, _ = v.stride()
-        rc = self.lib.rans_kv_append(self._p, k.data_ptr(), v.data_ptr(), given, kt * size, kh * size, vt * size, vh * size,
-                                     self._starts(starts, n), n, self._stream())
+        given, k_usable, v_usable, kt, kh, vt, vh = known
+        if k.get_device() != self._index or v.get_device() != self._index:
+            raise ValueError(f"k and v must be on {self.device}")
+        n, row = k.shape[0], self.dim * (4 if given == _FP32 else 2)
+        if not k_usable or k.data_ptr() % 16:
+            k, kt, kh = self._aligned(k, k_usable), self.kv_heads * row, row
+        if not v_usable or v.data_ptr() % 16:
+            v, vt, vh = self._aligned(v, v_usable), self.kv_heads * row, row
+        rc = self.lib.rans_kv_append(self._p, k.data_ptr(), v.data_ptr(), given, kt, kh, vt, vh, self._starts(starts, n), n,
+                                     self._stream())
         rb._check(rc, "rans_kv_append")
 
     def read(self, starts=None, tokens=None):
@@ -271,28 +276,31 @@ class KVCache:
         known = self._sizes.get(key)
         if known is None:
             known = self._sizes[key] = self._query(q, weigh)
-        kind, heads, usable = known
-        _need(q.get_device() == self._index, f"q must be on {self.device}")
-        q = self._aligned(q, usable)
+        kind, heads, usable, q_batch, q_head, sums = known
+        if q.get_device() != self._index:
+            raise ValueError(f"q must be on {self.device}")
+        if not usable or q.data_ptr() % 16:
+            q = self._aligned(q, usable)
+            q_batch, q_head = heads * self.dim * 2, self.dim * 2
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             _need(out.shape == q.shape and out.dtype == q.dtype and out.device == self.device and out.is_contiguous()
                   and out.data_ptr() % 16 == 0, "out must be contiguous and like q")
         if log_sum is None:
-            log_sum = torch.empty((self.batch, heads), dtype=torch.float32, device=self.device)
+            log_sum = torch.empty_like(sums)
         else:
             _need(log_sum.shape == (self.batch, heads) and log_sum.dtype == torch.float32 and log_sum.device == self.device
                   and log_sum.is_contiguous(), "log_sum must be contiguous fp32 [batch, heads]")
-        q_batch, q_head, _ = q.stride()
-        rc = self.lib.rans_kv_attend(self._p, q.data_ptr(), kind, q_batch * 2, q_head * 2, heads,
+        rc = self.lib.rans_kv_attend(self._p, q.data_ptr(), kind, q_batch, q_head, heads,
                                      self.dim ** -0.5 if scale is None else scale, out.data_ptr(), log_sum.data_ptr(),
                                      1 if weigh else 0, self._stream())
         rb._check(rc, "rans_kv_attend")
         return out, log_sum
 
     def _query(self, q, weigh):
-        """Checks of attend's query, which depend on its shape alone, and the workspace for it."""
+        """Checks of attend's query, which depend on its shape alone, and the workspace for it: (type, heads, strides are
+        usable, strides in bytes, a tensor like log_sum)."""
         torch = self._torch
         _need(q.dim() == 3 and q.shape[0] == self.batch and q.shape[2] == self.dim and q.device == self.device
               and q.shape[1] > 0 and q.shape[1] % self.kv_heads == 0,
@@ -304,7 +312,8 @@ class KVCache:
         size = self.lib.rans_kv_attend_bytes(self._p, q.shape[1], int(weigh))
         _need(size > 0, f"{q.shape[1]} query heads on {self.kv_heads}, or the table's size, are more than the kernel counts")
         self._room(size)
-        return kind, q.shape[1], q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0
+        return (kind, q.shape[1], q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0, q.stride(0) * 2,
+                q.stride(1) * 2, torch.empty((self.batch, q.shape[1]), dtype=torch.float32, device=self.device))
 
     def evict(self, budget, recent=0):
         """Bring sequences with more than `budget` tokens back to it, per kv head: the `recent` newest tokens and the
@@ -312,7 +321,7 @@ class KVCache:
         pages past the budget come back (to this cache's free list, or to the caller who hands them out)."""
         _need(self.weight is not None and self.position is not None, "this cache has no weight and position tensors")
         budget, recent = int(budget), int(recent)
-        _need(budget >= 1 and 0 <= recent <= budget, "budget >= 1 and 0 <= recent <= budget")
+        _need(budget >= 1 and 0 <= recent <= budget, "budget must be positive and recent between 0 and budget")
         size = self._sizes.get(budget)
         if size is None:
             size = self._sizes[budget] = self.lib.rans_kv_evict_bytes(self._p, budget)
