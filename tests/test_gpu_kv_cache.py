@@ -35,7 +35,7 @@ def rc():
     return rans_cache
 
 
-def fill(torch, rc, lens, kv_heads, dim, page, kind, seed=0, spread=1.0, tail=2, layout="head", special=False):
+def fill(torch, rc, lens, kv_heads, dim, page, kind, seed=0, spread=1.0, tail=2, layout="head", exponents=None):
     """A cache over tensors whose unused slots and pages hold NaN, and the stored rows of each sequence in 64 bits."""
     rng = np.random.default_rng(seed)
     need = [-(-n // page) for n in lens]
@@ -57,7 +57,12 @@ def fill(torch, rc, lens, kv_heads, dim, page, kind, seed=0, spread=1.0, tail=2,
             for i in range(need[b]):
                 used[table[b, i], :min(page, n - i * page)] = True
         if kind == "mxfp4":
-            full = full * np.exp2(rng.integers(-6, 7, (pages, kv_heads, page, dim // 32)).repeat(32, -1))
+            e = rng.integers(-6, 7, (pages, kv_heads, page, dim // 32))
+            if name == "v" and exponents is not None:
+                for b, n in enumerate(lens):
+                    for t in range(n):
+                        e[table[b, t // page], :, t % page] = exponents(rng, t, e.shape[1::2])
+            full = full * np.exp2(e.repeat(32, -1))
             index, scale = orc.quantise(full)
             stored = orc.values(index, scale)
             scale[~used[:, None, :].repeat(kv_heads, 1)] = 255
@@ -85,7 +90,7 @@ def fill(torch, rc, lens, kv_heads, dim, page, kind, seed=0, spread=1.0, tail=2,
     return cache, truth, table
 
 
-def check_attend(torch, cache, truth, q, lens, scale, got, weight=None, table=None, before=0.0):
+def check_attend(torch, cache, truth, q, lens, scale, got, weight=None, table=None, before=0.0, floor=0.0):
     out, log_sum = got[0].double().cpu().numpy(), got[1].double().cpu().numpy()
     qn = q.double().cpu().numpy()
     u_out = FP16 if q.dtype == torch.float16 else BF16
@@ -103,6 +108,7 @@ def check_attend(torch, cache, truth, q, lens, scale, got, weight=None, table=No
         bound = (u_p + u_out + 2 * delta + 2.0 ** -20) * size
         if cache.kind == "fp16":
             bound = bound + n * 2.0 ** -25 * np.abs(v).max()
+        bound = bound + floor * np.repeat(np.abs(v).sum(1), group, axis=0)
         bound = bound + n * 2.0 ** -126 * np.abs(v).max() + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -133)
         assert (np.abs(out[b] - want) <= bound).all(), (b, n, (np.abs(out[b] - want) / bound).max())
         assert np.abs(log_sum[b] - ls).max() <= delta + 2.0 ** -20 * (1 + np.abs(ls).max())
@@ -150,6 +156,31 @@ def test_attend_over_4_bits_takes_both_query_types(torch, rc, q_type):
     q = (torch.randn(2, 8, 128, device="cuda") * torch.tensor([[[1e-3]], [[100.0]]], device="cuda"))
     q = q.to(torch.float16 if q_type == "fp16" else torch.bfloat16)
     check_attend(torch, cache, truth, q, lens, 0.01, cache.attend(q, scale=0.01))
+
+
+APART = {
+    "far apart": lambda rng, t, shape: rng.integers(-60, 60, shape),
+    "rising": lambda rng, t, shape: np.full(shape, min(-50 + t // 3, 55)),
+    "falling": lambda rng, t, shape: np.full(shape, max(50 - t // 3, -55)),
+    "one large": lambda rng, t, shape: np.full(shape, 40 if t == 37 else -1),
+    "one small": lambda rng, t, shape: np.full(shape, -50 if t == 21 else 2),
+    "blocks apart": lambda rng, t, shape: np.broadcast_to(np.arange(shape[1]) * 12 - 20, shape),
+    "zeros": lambda rng, t, shape: np.full(shape, -63 if t % 2 else 3),
+}
+
+
+@pytest.mark.parametrize("exponents", list(APART))
+@pytest.mark.parametrize("dim,heads", [(64, 4), (128, 8), (128, 24), (256, 8)])
+def test_attend_over_4_bit_values_of_very_different_scales(torch, rc, exponents, dim, heads):
+    """Tiles inside and outside what fp16 operands take, in both directions, and the units that O is held in.  Probabilities
+    in fp16 are whole multiples of 2^-24 where the largest is at least 2^11 (the kernel keeps it between 2^0 and 2^15, and
+    above 2^11 at the last rise): each is off by up to 2^-36 of the largest, which shows where the tokens that dominate hold
+    zeros in a column."""
+    lens = [45, 333, 16, 1]
+    cache, truth, table = fill(torch, rc, lens, 2, dim, 16, "mxfp4", seed=dim, exponents=APART[exponents])
+    q = torch.randn(len(lens), heads, dim, device="cuda").bfloat16()
+    got = cache.attend(q, scale=0.05, weigh=True)
+    check_attend(torch, cache, truth, q, lens, 0.05, got, cache.weight, table, floor=2.0 ** -36)
 
 
 @pytest.mark.parametrize("layout", ["token", "wide"])
