@@ -227,6 +227,11 @@ class KVCache:
     def free_pages(self):
         return len(self._free)
 
+    @property
+    def most(self):
+        """What the host knows of the lengths: no sequence is longer than this (pages reserved, less what evict gave back)."""
+        return list(self._most)
+
     def nbytes(self):
         """Bytes of rows, scales and books."""
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.weight, self.position)

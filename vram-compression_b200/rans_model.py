@@ -18,6 +18,9 @@ next steps in its README.  This module connects the two ends:
                                  step in-kernel), larger batches decode to bf16
                                  and use a dense GEMM; escapes completed by
                                  rans_escape_gemv / rans_escape_decode
+  RansAttention                  torch module: the attention block of a decoder layer for one
+                                 new token per sequence, its projections entropy coded and
+                                 its keys and values in a rans_cache.KVCache
 
 Everything that touches the GPU goes through librans_b200.so; there is no CPU
 fallback.
@@ -321,3 +324,45 @@ class RansLinear(_torch_nn().nn.Module):
         if self.bias is not None:
             y = y + self.bias
         return y.to(x.dtype).reshape(*lead, self.out_features)
+
+
+class RansAttention(_torch_nn().nn.Module):
+    """The attention block of a decoder layer, one new token per sequence: q, k, v products from entropy-coded weights
+    (RansLinear), the token's keys and values into a paged cache (16-bit or 4-bit), attention over the cache, the o product.
+
+    cache: a rans_cache.KVCache with the layer's kv heads, head size and as many sequences as x has rows.  rotate:
+    optional callable (q, k, seen) -> (q, k) for positional rotation; q [batch, heads, dim], k [batch, kv_heads, dim],
+    seen the tokens that each sequence had before (int32, on the device).  budget: keep at most this many tokens of a
+    sequence, the `recent` newest and those that received most attention; checked after every token, and done once a
+    sequence may hold `slack` tokens more than that.
+    """
+
+    def __init__(self, q, k, v, o, cache, heads, scale=None, rotate=None, budget=None, recent=0, slack=0):
+        super().__init__()
+        kv = cache.kv_heads * cache.dim
+        if (q.out_features, k.out_features, v.out_features, o.in_features) != (heads * cache.dim, kv, kv, heads * cache.dim):
+            raise ValueError("projections do not fit the heads of the cache")
+        if heads % cache.kv_heads:
+            raise ValueError("heads must be a multiple of the cache's kv_heads")
+        if budget is not None and (budget < 1 or not 0 <= recent <= budget or slack < 0):
+            raise ValueError("budget must be positive, recent between 0 and budget, slack not negative")
+        self.q, self.k, self.v, self.o = q, k, v, o
+        self.cache, self.heads, self.scale, self.rotate = cache, heads, scale, rotate
+        self.budget, self.recent, self.slack = budget, recent, slack
+
+    def forward(self, x):
+        """x [batch, hidden], the new token of every sequence -> [batch, hidden]."""
+        torch, c = rb._torch(), self.cache
+        if x.dim() != 2 or x.shape[0] != c.batch:
+            raise ValueError(f"expected [{c.batch}, hidden], got {tuple(x.shape)}")
+        q = self.q(x).view(c.batch, self.heads, c.dim)
+        k, v = (p(x).view(c.batch, c.kv_heads, c.dim) for p in (self.k, self.v))
+        if self.rotate is not None:
+            q, k = self.rotate(q, k, c.seen)
+        c.reserve([1] * c.batch)
+        c.append(k, v)
+        out, _ = c.attend(q.to(torch.float16 if c.kind == "fp16" else torch.bfloat16), scale=self.scale,
+                          weigh=self.budget is not None)
+        if self.budget is not None and max(c.most) > self.budget + self.slack:
+            c.evict(self.budget, self.recent)
+        return self.o(out.view(c.batch, -1)).to(x.dtype)
