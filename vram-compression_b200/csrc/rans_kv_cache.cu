@@ -19,11 +19,13 @@ constexpr int kThreads = 256;
 
 // ------------------------------------------------------------------ append, read
 // One thread per 8 values of a row: 16 bytes of a 16-bit row, one word of a 4-bit
-// row (a quarter of a block of 32, so four neighbouring lanes share a scale).
+// row (a quarter of a block of 32, so four neighbouring lanes share a scale).  A
+// thread keeps its column (head and part of the row) and goes through the block's
+// tokens, whose places are found once: what is left per 8 values is the rounding.
 
 struct RowArgs {
     RansKvCache c;
-    Divider page, heads;
+    Divider page;
     const char* k_in;
     const char* v_in;
     int64_t k_token, k_head, v_token, v_head;      // bytes
@@ -32,14 +34,17 @@ struct RowArgs {
     const int32_t* starts;
     int tokens;
     int part_shift;                                // log2 of a row's threads
+    Divider columns;                               // by the threads of one token, or the block's if they are fewer
 };
 
 // Tokens of a block: a warp each to find out where they are.
 constexpr int kTokens = kThreads / 32;
 
 struct Where {
-    int page, slot;            // page -1: nowhere
-    int b, position;
+    int64_t k, v;              // where the token's first key and value row lies, in bytes
+    int64_t place;             // and its books: of head 0
+    int position;
+    int ok;                    // 0: nowhere
 };
 
 __device__ __forceinline__ int rows_of(const RowArgs& a, int b) {
@@ -72,7 +77,7 @@ __device__ __forceinline__ void find_tokens(const RowArgs& a, Where* where, bool
         int first;
         const int b = sequence_of(a, token, lane, first);
         if (lane == 0) {
-            Where w{-1, 0, b, 0};
+            Where w{};
             if (b < 0) {
                 raise(c, RANS_KV_BAD_STARTS);
             } else {
@@ -84,9 +89,13 @@ __device__ __forceinline__ void find_tokens(const RowArgs& a, Where* where, bool
                 } else if (place >= (int64_t)c.table_cols * c.page) {
                     raise(c, RANS_KV_BAD_LENGTH);
                 } else {
-                    const int in_page = a.page(place);
-                    w.page = checked_page(c, b, in_page);
-                    w.slot = place - in_page * c.page;
+                    const int in_page = a.page(place), page = checked_page(c, b, in_page), slot = place - in_page * c.page;
+                    if (page >= 0) {
+                        w.ok = 1;
+                        w.k = page * c.k_page + slot * c.k_slot;
+                        w.v = page * c.v_page + slot * c.v_slot;
+                        w.place = (int64_t)page * c.kv_heads * c.page + slot;
+                    }
                 }
             }
             where[warp] = w;
@@ -139,14 +148,45 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8], int kind) {
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// 8 values in the cache's 16-bit type.
+template <int GIVEN>
+__device__ __forceinline__ uint4 rounded8(const Given8<GIVEN>& y, int kind) {
+    if (kind == GIVEN) return y.w[0];
+    float x[8];
+    to_float(x, y);
+    return pack8(x, kind);
+}
+
+// Four pairs of values as e2m1 codes, the first of a pair in a byte's low half.
+__device__ __forceinline__ uint32_t to_e2m1(const float (&x)[8]) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+    return r;
+}
+
 // 8 values of a block of 32 that lies over 4 neighbouring lanes -> 8 codes; `byte` the block's scale.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& byte) {
-    // magnitudes compare as integers, and an infinity or NaN as the largest
-    uint32_t top = 0;
+template <int GIVEN>
+__device__ __forceinline__ uint32_t quantise8(const Given8<GIVEN>& y, uint32_t& byte) {
+    float x[8];
+    uint32_t top;          // the largest magnitude's bits: magnitudes compare as integers, an infinity or NaN as the largest
+    if constexpr (GIVEN == RANS_KV_BF16) {
+        const uint32_t abs = 0x7fff7fffu;
+        uint32_t m = __vmaxu2(__vimax3_u16x2(y.w[0].x & abs, y.w[0].y & abs, y.w[0].z & abs), y.w[0].w & abs);
+        m = __vmaxu2(m, __shfl_xor_sync(~0u, m, 1));
+        m = __vmaxu2(m, __shfl_xor_sync(~0u, m, 2));
+        top = max(m & 0xffff0000u, m << 16);
+    } else {
+        to_float(x, y);
+        top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(~0u, top, 1));
-    top = max(top, __shfl_xor_sync(~0u, top, 2));
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(~0u, top, 1));
+        top = max(top, __shfl_xor_sync(~0u, top, 2));
+    }
     if (top >= 0x7f800000u) {
         byte = 255;
         return 0;
@@ -154,11 +194,10 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& byt
     const int e = min(max((int)(top >> 23) - 127 - 2, -63), 63);
     byte = (uint32_t)(e + 127);
     const float f = __uint_as_float((uint32_t)(127 - e) << 23);      // 2^-e: the division is exact
-    uint32_t code = 0;
+    if constexpr (GIVEN == RANS_KV_BF16) to_float(x, y);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        code |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] * f, x[2 * i + 1] * f), __NV_E2M1, cudaRoundNearest) << (8 * i);
-    return code;
+    for (int i = 0; i < 8; ++i) x[i] *= f;
+    return to_e2m1(x);
 }
 
 template <int GIVEN>
@@ -168,22 +207,30 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     const RansKvCache& c = a.c;
     wait_for_previous();
     let_next_start();
-    const int per_row = 1 << a.part_shift, tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens);
-    const int all = (tokens * c.kv_heads) << a.part_shift;
+    const int tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens), columns = c.kv_heads << a.part_shift;
+    const int wide = min(columns, kThreads), t0 = a.columns(threadIdx.x), c0 = threadIdx.x - t0 * wide, step = a.columns(kThreads);
     constexpr int kAtOnce = GIVEN == RANS_KV_FP32 ? 2 : 4;
     Given8<GIVEN> in[kAtOnce][2];
-    auto load = [&](int i0) {
+    // token t0 + (first + u) * step of the block, column `col`; threads beyond step * wide have no token
+    auto token_of = [&](int first, int u, int col) {
+        const int t = t0 + (first + u) * step;
+        return t0 < step && col < columns && t < tokens ? t : -1;
+    };
+    auto load = [&](int first, int col) {
+        const int h = col >> a.part_shift;
+        const int64_t at = (int64_t)(col & ((1 << a.part_shift) - 1)) * sizeof(Given8<GIVEN>);
+        const char *k = a.k_in + h * a.k_head + at, *v = a.v_in + h * a.v_head + at;
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
+            const int t = token_of(first, u, col);
             in[u][0] = in[u][1] = Given8<GIVEN>{};
-            if (i >= all) continue;
-            const int64_t token = blockIdx.x * kTokens + t, at = (int64_t)part * sizeof(Given8<GIVEN>);
-            load8(in[u][0], a.k_in + token * a.k_token + h * a.k_head + at);
-            load8(in[u][1], a.v_in + token * a.v_token + h * a.v_head + at);
+            if (t < 0) continue;
+            const int64_t token = blockIdx.x * kTokens + t;
+            load8(in[u][0], k + token * a.k_token);
+            load8(in[u][1], v + token * a.v_token);
         }
     };
-    load(threadIdx.x);                             // on their way while the block finds out where they go
+    load(0, c0);                                   // on their way while the block finds out where they go
     find_tokens(a, where, false);
     // The block has read its lengths; the last one to say so moves them on below.
     int* counter = static_cast<int*>(c.workspace);
@@ -191,37 +238,41 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         last = atomicAdd(counter, 1) == (int)gridDim.x - 1;
         if (last) *counter = 0;
     }
-    // (a row has 8 threads or more, so the four lanes of a block of 32 values are in or out of range together)
-    for (int i0 = threadIdx.x; i0 - (int)(threadIdx.x & 31) < all; i0 += kThreads * kAtOnce) {
-        if (i0 != (int)threadIdx.x) load(i0);
+    // (all lanes take every turn: a row has 8 threads or more, so a block of 32 values lies in four lanes that have a token
+    // or none together)
+    for (int col0 = 0; col0 < columns; col0 += wide) {
+        const int col = c0 + col0, h = col >> a.part_shift, part = col & ((1 << a.part_shift) - 1);
+        char *k = static_cast<char*>(c.k) + h * c.k_head, *v = static_cast<char*>(c.v) + h * c.v_head;
+        const int in_row = c.kind == RANS_KV_MXFP4 ? (part % 4 << a.part_shift) + part / 4 * 4 : part * 16;
+        for (int first = 0; first * step < tokens; first += kAtOnce) {
+            if (col0 != 0 || first != 0) load(first, col);
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
-            if (i - (int)(threadIdx.x & 31) >= all) break;
-            const Where w = where[i < all ? t : 0];
-            const bool stored = i < all && w.page >= 0;
-            const int64_t place = ((int64_t)w.page * c.kv_heads + h) * c.page + w.slot;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                float x[8];
-                to_float(x, in[u][v]);
-                char* base = static_cast<char*>(v == 0 ? c.k : c.v);
-                const int64_t at = w.page * (v == 0 ? c.k_page : c.v_page) + h * (v == 0 ? c.k_head : c.v_head) + w.slot * (v == 0 ? c.k_slot : c.v_slot);
+            for (int u = 0; u < kAtOnce; ++u) {
+                if ((first + u) * step >= tokens) break;
+                const int t = token_of(first, u, col);
+                const Where& w = where[max(t, 0)];
+                const bool stored = t >= 0 && w.ok;
+                const int64_t place = w.place + h * c.page;
                 if (c.kind == RANS_KV_MXFP4) {
-                    uint32_t byte;
-                    const uint32_t code = quantise8(x, byte);
+                    uint32_t byte[2];
+                    const uint32_t k_code = quantise8(in[u][0], byte[0]), v_code = quantise8(in[u][1], byte[1]);
                     if (stored) {
-                        const int n = part / 4, q = part % 4;
-                        *reinterpret_cast<uint32_t*>(base + at + q * per_row + n * 4) = code;
-                        if (q == 0) (v == 0 ? c.k_scale : c.v_scale)[place * (c.dim / 32) + n] = (uint8_t)byte;
+                        *reinterpret_cast<uint32_t*>(k + w.k + in_row) = k_code;
+                        *reinterpret_cast<uint32_t*>(v + w.v + in_row) = v_code;
+                        if (part % 4 == 0) {
+                            const int64_t at = (place << (a.part_shift - 2)) + part / 4;
+                            c.k_scale[at] = (uint8_t)byte[0];
+                            c.v_scale[at] = (uint8_t)byte[1];
+                        }
                     }
                 } else if (stored) {
-                    *reinterpret_cast<uint4*>(base + at + part * 16) = pack8(x, c.kind);
+                    *reinterpret_cast<uint4*>(k + w.k + in_row) = rounded8(in[u][0], c.kind);
+                    *reinterpret_cast<uint4*>(v + w.v + in_row) = rounded8(in[u][1], c.kind);
                 }
-            }
-            if (stored && part == 0) {
-                if (c.position != nullptr) c.position[place] = w.position;
-                if (c.weight != nullptr) c.weight[place] = 0.0f;
+                if (stored && part == 0) {
+                    if (c.position != nullptr) c.position[place] = w.position;
+                    if (c.weight != nullptr) c.weight[place] = 0.0f;
+                }
             }
         }
     }
@@ -234,58 +285,61 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         }
 }
 
+// What 8 codes and their block's scale byte stand for, in bf16 (exact).
+__device__ __forceinline__ uint4 values8(uint32_t code, uint32_t byte) {
+    const float f = byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const __half2_raw r = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((code >> (8 * e)) & 255), __NV_E2M1);
+        const float2 z = __half22float2(__half2(r));
+        y[2 * e] = z.x * f;
+        y[2 * e + 1] = z.y * f;
+    }
+    return pack8(y, RANS_KV_BF16);
+}
+
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ RowArgs a) {
     __shared__ Where where[kTokens];
     const RansKvCache& c = a.c;
     wait_for_previous();
     let_next_start();
     find_tokens(a, where, true);
-    const int per_row = 1 << a.part_shift, tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens);
-    const int all = (tokens * c.kv_heads) << a.part_shift;
-    const int64_t out0 = ((int64_t)blockIdx.x * kTokens * c.kv_heads) << a.part_shift;
-    constexpr int kAtOnce = 2;
-    for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kAtOnce) {
-        uint4 x[kAtOnce][2];               // 4 bits: the codes in .x, the scale byte in .y
+    const int tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens), columns = c.kv_heads << a.part_shift;
+    const int wide = min(columns, kThreads), t0 = a.columns(threadIdx.x), c0 = threadIdx.x - t0 * wide, step = a.columns(kThreads);
+    if (t0 >= step) return;
+    const int64_t out0 = (int64_t)blockIdx.x * kTokens * columns;
+    constexpr int kAtOnce = 4;
+    for (int col = c0; col < columns; col += wide) {
+        const int h = col >> a.part_shift, part = col & ((1 << a.part_shift) - 1);
+        const char *k = static_cast<const char*>(c.k) + h * c.k_head, *v = static_cast<const char*>(c.v) + h * c.v_head;
+        for (int first = t0; first < tokens; first += step * kAtOnce) {
+            uint4 x[kAtOnce][2];           // 4 bits: the codes in .x, the scale byte in .y
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kThreads, part = i & (per_row - 1), row = i >> a.part_shift, t = a.heads(row), h = row - t * c.kv_heads;
-            x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
-            if (i >= all) continue;
-            const Where w = where[t];
-            if (w.page < 0) continue;
-            const int64_t place = ((int64_t)w.page * c.kv_heads + h) * c.page + w.slot;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const char* base = static_cast<const char*>(v == 0 ? c.k : c.v) + w.page * (v == 0 ? c.k_page : c.v_page) +
-                                   h * (v == 0 ? c.k_head : c.v_head) + w.slot * (v == 0 ? c.k_slot : c.v_slot);
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int t = first + u * step;
+                x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
+                if (t >= tokens || !where[t].ok) continue;
+                const Where& w = where[t];
                 if (c.kind == RANS_KV_MXFP4) {
-                    x[u][v].x = *reinterpret_cast<const uint32_t*>(base + part % 4 * per_row + part / 4 * 4);
-                    x[u][v].y = (v == 0 ? c.k_scale : c.v_scale)[place * (c.dim / 32) + part / 4];
+                    const int in_row = (part % 4 << a.part_shift) + part / 4 * 4;
+                    const int64_t at = ((w.place + h * c.page) << (a.part_shift - 2)) + part / 4;
+                    x[u][0].x = *reinterpret_cast<const uint32_t*>(k + w.k + in_row);
+                    x[u][0].y = c.k_scale[at];
+                    x[u][1].x = *reinterpret_cast<const uint32_t*>(v + w.v + in_row);
+                    x[u][1].y = c.v_scale[at];
                 } else {
-                    x[u][v] = *reinterpret_cast<const uint4*>(base + part * 16);
+                    x[u][0] = *reinterpret_cast<const uint4*>(k + w.k + part * 16);
+                    x[u][1] = *reinterpret_cast<const uint4*>(v + w.v + part * 16);
                 }
             }
-        }
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kThreads;
-            if (i >= all) continue;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                uint4 out = x[u][v];
-                if (c.kind == RANS_KV_MXFP4) {
-                    const float f = out.y == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(out.y << 23);
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const __half2_raw r = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((out.x >> (8 * e)) & 255), __NV_E2M1);
-                        const float2 z = __half22float2(__half2(r));
-                        y[2 * e] = z.x * f;
-                        y[2 * e + 1] = z.y * f;
-                    }
-                    out = pack8(y, RANS_KV_BF16);
-                }
-                (v == 0 ? a.k_out : a.v_out)[out0 + i] = out;
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int t = first + u * step;
+                if (t >= tokens) continue;
+                const int64_t at = out0 + (int64_t)t * columns + col;
+                a.k_out[at] = c.kind == RANS_KV_MXFP4 ? values8(x[u][0].x, x[u][0].y) : x[u][0];
+                a.v_out[at] = c.kind == RANS_KV_MXFP4 ? values8(x[u][1].x, x[u][1].y) : x[u][1];
             }
         }
     }
@@ -662,10 +716,11 @@ void set_rows(RowArgs& a, const RansKvCache& c, const int32_t* starts, int token
     a.c = c;
     fill_strides(a.c);
     a.page = Divider::of((uint32_t)c.page);
-    a.heads = Divider::of((uint32_t)c.kv_heads);
     a.starts = starts;
     a.tokens = tokens;
     a.part_shift = c.dim == 64 ? 3 : c.dim == 128 ? 4 : 5;
+    const int columns = c.kv_heads << a.part_shift;
+    a.columns = Divider::of((uint32_t)(columns < kThreads ? columns : kThreads));
 }
 
 int row_grid(const RowArgs& a) { return (a.tokens + kTokens - 1) / kTokens; }
