@@ -18,7 +18,8 @@
 // key row are its operands of two consecutive k-steps, with
 // Q's registers loaded in the same order; and a lane that reads the same 8
 // columns of four value rows gets V^T's operands by one byte permute each.
-// Nothing is staged, so no warp waits for another while it streams.
+// Nothing is staged, so no warp waits for another while it streams.  4-bit rows are
+// staged instead (their loop is bound by instructions and has no registers to spare).
 //
 // Work is shared out by tiles: the grid's warps get equal runs of the list of all
 // (sequence, kv head, tile), whatever the lengths are.  A warp that has a whole
@@ -26,6 +27,12 @@
 // shared memory, and the last block to finish a (sequence, kv head) joins the
 // blocks' parts (always in the order of the tiles, so results do not depend on
 // which block that is).
+//
+// Measured on one B200, 64 query heads on 8 of size 128: 48 uneven sequences in bf16
+// (1.58 GB) 235 us, 6.7 TB/s, the rate of a plain copy; one of 32768 tokens 30 us, of
+// which 18 us stream at 7.3 TB/s and the rest is launch, page lookups and joins; one of
+// 131071 tokens in 4 bits (143 MB) 48 us, about 420 instructions per 16 tokens; one of
+// 777 tokens on 2 heads 8.6 us.
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -1161,7 +1168,8 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
 }
 
 // weight[t] += sum over a kv head's query heads of exp2(score - m) / l.  A warp takes 64 tokens of a head at a time, each lane
-// two of them: scores are read 32 bytes a lane, the heads' m and 1 / l by one lane each.
+// two of them: scores are read 32 bytes a lane, the heads' m and 1 / l by one lane each.  Bound by reading the scores (4 bytes
+// a token and query head, mostly from L2): with the stores of attend_kernel 11 us of a step of 16 x 4097 tokens on 64 heads.
 constexpr int kWeighThreads = 256;
 constexpr int kSpan = 64;
 constexpr int kWeighBlocks = 6;          // an SM

@@ -22,6 +22,8 @@ constexpr int kThreads = 256;
 // row (a quarter of a block of 32, so four neighbouring lanes share a scale).  A
 // thread keeps its column (head and part of the row) and goes through the block's
 // tokens, whose places are found once: what is left per 8 values is the rounding.
+// 10127 tokens of 8 heads of 128 into 4 bits and back: 30 us together, bound by
+// instructions; one token each of 4 sequences 2.8 us.
 
 struct RowArgs {
     RansKvCache c;
@@ -350,7 +352,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 // keys (passes of 11, 11 and 10 bits, of which the last is seldom needed; the blocks' histograms are added up through the
 // cluster's shared memory), mark what stays, pair
 // the i-th kept place at or above the budget with the i-th freed place below it, and move the rows.  Sources lie at or above
-// the budget and destinations below it, so moves never meet.
+// the budget and destinations below it, so moves never meet.  Bound by the passes' latency (32 x 2 heads of 4160 tokens: 12 us)
+// and, where much moves, by rows of 256 bytes read and written (8 heads of 65536 to 16384, 50 MB: 22 us to select, 24 to move).
 
 constexpr int kSelect = 1024;
 constexpr int kSelectWarps = kSelect / 32;
