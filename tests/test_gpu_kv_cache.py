@@ -35,13 +35,13 @@ def rc():
     return rans_cache
 
 
-def fill(torch, rc, lens, kv_heads, dim, page, kind, seed=0, spread=1.0, tail=2, layout="head", exponents=None):
+def fill(torch, rc, lens, kv_heads, dim, page, kind, seed=0, spread=1.0, tail=2, layout="head", exponents=None, cols=1):
     """A cache over tensors whose unused slots and pages hold NaN, and the stored rows of each sequence in 64 bits."""
     rng = np.random.default_rng(seed)
     need = [-(-n // page) for n in lens]
     pages = sum(need) + tail
     order = rng.permutation(pages)
-    cols = max(max(need), 1) + 1
+    cols = max(max(need) + 1, cols)
     table = np.full((len(lens), cols), -1, np.int32)
     at = 0
     for b, m in enumerate(need):
@@ -332,8 +332,8 @@ def test_append_4_bits_of_every_kind_of_block(torch, rc):
 
 
 # ------------------------------------------------------------------ evict
-def _evict_case(torch, rc, lens, kv_heads, dim, page, kind, weights, budget, recent, seed=0):
-    cache, truth, table = fill(torch, rc, lens, kv_heads, dim, page, kind, seed=seed)
+def _evict_case(torch, rc, lens, kv_heads, dim, page, kind, weights, budget, recent, seed=0, cols=1):
+    cache, truth, table = fill(torch, rc, lens, kv_heads, dim, page, kind, seed=seed, cols=cols)
     rng = np.random.default_rng(seed)
     w = np.full(cache.weight.shape, np.nan, np.float32)
     pos = np.full(cache.weight.shape, 1 << 30, np.int32)
@@ -405,6 +405,19 @@ def test_evict_kinds(torch, rc, kind, dim, page):
 @pytest.mark.parametrize("n,budget", [(20000, 5000), (33333, 33332), (60000, 1)])
 def test_evict_long(torch, rc, n, budget):
     _evict_case(torch, rc, [n], 1, 64, 64, "bf16", SOME["random"], budget, min(64, budget))
+
+
+@pytest.mark.parametrize("kind,dim", [("bf16", 256), ("fp16", 256)])
+def test_evict_many_rows_of_few_heads(torch, rc, kind, dim):
+    """Enough rows for the moves to get a grid of their own (32 MB over 8 heads, by the table's room)."""
+    _evict_case(torch, rc, [6000], 8, dim, 64, kind, SOME["random"], 4096, 64, cols=129)
+
+
+@pytest.mark.parametrize("weights", ["random", "few values"])
+def test_evict_with_keys_in_the_workspace(torch, rc, weights):
+    """More places in the table than a block's shared memory has keys for, over more heads than there are SMs for clusters."""
+    _evict_case(torch, rc, [150, 33, 0], 30, 64, 16, "bf16", SOME[weights], 50, 10, cols=2700)
+    _evict_case(torch, rc, [52], 150, 64, 16, "bf16", SOME[weights], 50, 10, cols=2700)
 
 
 def test_evicting_again_moves_nothing(torch, rc):

@@ -167,8 +167,11 @@ struct Attend {
     static constexpr bool kFp4 = KIND == RANS_KV_MXFP4;
     static constexpr int HP = NT * 8;                         // heads of a tile, padded
     static constexpr int kChunks = D / 32;                    // 32 values of a row
-    // One block of an SM's whole register file: fewer parts to join than from several blocks.
-    static constexpr int kWarps = (NT == 2 && D == 128) || D == 256 ? 8 : D == 128 && !kFp4 ? 12 : 16;
+    // One block of an SM's whole register file: fewer parts to join than from several blocks.  As many warps as the registers
+    // for rows, O and statistics allow without spilling; 4-bit rows are not held in registers (12 against 8 warps: 16 x 8000
+    // tokens of 8 heads in 4 bits, groups of 12 heads of 128: 79 -> 68 us, of 8 heads of 256: 93 -> 83 us).
+    static constexpr bool kLarge = (NT == 2 && D == 128) || D == 256;
+    static constexpr int kWarps = kLarge ? (kFp4 ? 12 : 8) : D == 128 && !kFp4 ? 12 : 16;
     static constexpr int kRow = D + 4;                        // a head's part in shared memory
 
     // What is left of a run of tiles of one group: O, and the running maximum and sum of each head; a warp's in shared
@@ -201,12 +204,6 @@ struct Attend {
         int warp_sum[kWarps];
         int pre[RANS_KV_MAX_BATCH + 1];      // places of one head in front of each sequence
     };
-
-    // The token of a tile that row g (and, 8 further, row g + 8) of S^T stands for, and the one that a lane's i-th value row
-    // is (rows 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of P^T).  4-bit rows are read from shared memory, where neighbours in either
-    // order have to lie in different halves of the banks.
-    static __device__ __forceinline__ int key_row(int g) { return kFp4 ? (g & 6) | (((g >> 1) + g) & 1) : g; }
-    static __device__ __forceinline__ int value_row(int q4, int i) { return key_row(2 * q4 + (i & 1)) + 8 * (i >> 1); }
 
     // One tile's rows in registers, 16 bits a value ..
     struct RawK {
@@ -336,7 +333,7 @@ struct Attend {
         const int g = lane >> 2, q4 = lane & 3;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = key_row(g) + 8 * i;
+            const int row = g + 8 * i;
             const uint8_t* p = st.k + row * (D / 2) + q4 * (D / 8);
             if constexpr (D == 64) {
                 const uint2 w = *reinterpret_cast<const uint2*>(p);
@@ -356,7 +353,7 @@ struct Attend {
         const int g = lane >> 2, q4 = lane & 3;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = value_row(q4, i);
+            const int row = 2 * q4 + (i & 1) + 8 * (i >> 1);
             const uint8_t* p = st.v + row * (D / 2) + g * (D / 16);
             const uint8_t* s = st.vs + row * kChunks + (g & 1) * (D / 64);
             if constexpr (D == 256) {
@@ -493,7 +490,7 @@ struct Attend {
     template <int SUB>
     static __device__ __forceinline__ void probabilities(State& s, float (&sc)[SUB][NT][4], const AttendArgs& a, int x,
                                                          const int (&valid)[SUB], int lane) {
-        const int q4 = lane & 3, row = key_row(lane >> 2);
+        const int q4 = lane & 3, row = lane >> 2;
         bool raise_max = false;
 #pragma unroll
         for (int i = 0; i < SUB; ++i)
@@ -615,7 +612,7 @@ struct Attend {
         for (int j = 0; j < D / 64; ++j) units |= (uint32_t)s.unit[j] << (8 * j);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (value_row(q4, i) >= valid) r.s[i] = units;
+            if (2 * q4 + (i & 1) + 8 * (i >> 1) >= valid) r.s[i] = units;
     }
 
     // O^T += V^T P^T over the first `count` of kSub tiles.
@@ -808,11 +805,11 @@ struct Attend {
             }
     }
 
-    // Joins four values of one head over n parts, in their order, eight parts' loads at once.  Every column's thread works
+    // Joins four values of one head over n parts, in their order, many parts' loads at once (8 groups over 148 blocks: two trips).  Every column's thread works
     // out the factors for itself: that costs a few exponentials, and no barrier and no second trip to memory.
     template <bool SHARED, class PartAt>
     static __device__ __forceinline__ void join(PartAt part_at, int n, int head, int d, float4& o, float& top, float& l) {
-        constexpr int kAtOnce = 8;
+        constexpr int kAtOnce = SHARED ? 8 : 10;
         o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         top = -INFINITY;
         l = 0.0f;
@@ -1152,10 +1149,10 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
         sm.last[tid] = last;
     }
     __syncthreads();
+    const int first_slices = sm.last[0] ? kSlices : 0, slices = first_slices + (sm.last[1] ? kSlices : 0);
 #pragma unroll 1
-    for (int v = tid; v < 2 * kVec; v += kThreads) {
-        const int i = v / kVec, head = v % kVec / (D / 4), d = v % (D / 4) * 4;
-        if (!sm.last[i]) continue;
+    for (int slice = warp; slice < slices; slice += W) {
+        const int i = slice < first_slices ? 0 : 1, v = (slice - (i == 0 ? 0 : first_slices)) * 32 + lane, head = v / (D / 4), d = v % (D / 4) * 4;
         const Group s = Group::of(i == 0 ? open0 : open1);
         if (head >= heads_of(s)) continue;
         const int nt = tiles_of(s.b), start = sm.pre[s.b] * segs + (s.h * a.subs + s.sub) * (nt + kStart);

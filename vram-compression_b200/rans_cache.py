@@ -20,7 +20,8 @@ or microscaled 4-bit rows (4.25 bits a value), and runs on it:
 Every method but reserve, release and check is one asynchronous call on the
 current stream (capturable in a CUDA graph once the workspace has its size: run it
 once before).  Calls on one cache share its books and workspace, so they have to be
-ordered: one stream, or events between streams.  Page numbers and lengths are
+ordered: one stream, or events between streams.  Sequences may share pages for attend
+alone; append, attend(weigh=True) and evict want every page in one place.  Page numbers and lengths are
 checked inside the kernels: what would lie outside is left out and check() raises.
 There is no CPU fallback.
 """
