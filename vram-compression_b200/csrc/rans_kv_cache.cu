@@ -355,9 +355,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 // the budget and destinations below it, so moves never meet.  Bound by the passes' latency (32 x 2 heads of 4160 tokens: 12 us)
 // and, where much moves, by rows of 256 bytes read and written (8 heads of 65536 to 16384, 50 MB: 22 us to select, 24 to move).
 
-constexpr int kSelect = 1024;
-constexpr int kSelectWarps = kSelect / 32;
-constexpr int kBins = 2048;                                // two per thread
+// Threads of a block: many for a head's latency, fewer where there are more heads than SMs, so that four blocks share one (392 heads
+// of 147 tokens 18.2 -> 7.3 us, of 4200 51.3 -> 37.6; 160 of 4200 28.6 -> 26.3; but 128 of 4160 16.2 -> 22.5).
+constexpr int kSelect = 1024, kSelectMany = 256;
+constexpr int kBins = 2048;
 constexpr int kFew = 4;                                    // tokens over the budget that are searched for one by one
 constexpr int kMaxCluster = 8;                             // the portable size; of 16, seven at most run at a time
 constexpr int kPlaces = 4096;                              // a block takes before there are more of them
@@ -443,14 +444,16 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, cons
             }
 }
 
-__global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ EvictArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ EvictArgs a) {
+    constexpr int kWarps = THREADS / 32, kPer = kBins / THREADS;
     extern __shared__ uint32_t shared_keys[];
     __shared__ __align__(8) int hist[2][kBins];
     __shared__ int digit_s, rank_s, count_s;
     __shared__ uint2 lightest[kFew];                       // the block's lightest token of each turn: key, place
-    __shared__ int wsum[2][kSelectWarps];
+    __shared__ int wsum[2][kWarps];
     __shared__ int block_sum[3];                           // ties, holes, movers of the block's places
-    __shared__ int4 moving[kSelect];                       // (page, slot) to and from
+    __shared__ int4 moving[THREADS];                       // (page, slot) to and from
     const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     const RansKvCache& c = a.c;
     const int blocks = cluster.num_blocks(), block = cluster.block_rank(), bh = blockIdx.x / blocks;
@@ -462,18 +465,18 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
     if (n > k) {
         // each block has a run of 32-place words, each warp a run of the block's
         const int words = (n + 31) / 32, bw0 = (int)((int64_t)words * block / blocks), bw1 = (int)((int64_t)words * (block + 1) / blocks);
-        const int w0 = bw0 + (bw1 - bw0) * warp / kSelectWarps, w1 = bw0 + (bw1 - bw0) * (warp + 1) / kSelectWarps;
+        const int w0 = bw0 + (bw1 - bw0) * warp / kWarps, w1 = bw0 + (bw1 - bw0) * (warp + 1) / kWarps;
         uint32_t* keys = a.keys != nullptr ? a.keys + (int64_t)bh * c.table_cols * c.page : shared_keys - (int64_t)bw0 * 32;
         const int first_late = c.seen[b] - a.recent;
         const int t_end = min(bw1 * 32, n);
         constexpr int kLoads = 4;
-        for (int t0 = bw0 * 32 + tid; t0 < t_end; t0 += kSelect * kLoads) {
+        for (int t0 = bw0 * 32 + tid; t0 < t_end; t0 += THREADS * kLoads) {
             int64_t at[kLoads];
             float weight[kLoads];
             int position[kLoads];
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int t = t0 + i * kSelect, in_page = a.page(t), p = t < t_end ? checked_page(c, b, in_page) : -1;
+                const int t = t0 + i * THREADS, in_page = a.page(t), p = t < t_end ? checked_page(c, b, in_page) : -1;
                 at[i] = p >= 0 ? ((int64_t)p * c.kv_heads + h) * c.page + (t - in_page * c.page) : -1;
             }
 #pragma unroll
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
             }
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                if (t0 + i * kSelect < t_end) keys[t0 + i * kSelect] = at[i] >= 0 ? key_of(weight[i], position[i] >= first_late) : 0;
+                if (t0 + i * THREADS < t_end) keys[t0 + i * THREADS] = at[i] >= 0 ? key_of(weight[i], position[i] >= first_late) : 0;
         }
         auto sync = [&]() {
             if (blocks == 1) __syncthreads(); else cluster.sync();
@@ -516,8 +519,8 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
                     wsum[1][warp] = last;
                 }
                 __syncthreads();
-                key = (uint32_t)wsum[0][lane];
-                place = wsum[1][lane];
+                key = lane < kWarps ? (uint32_t)wsum[0][lane] : 0xffffffffu;
+                place = lane < kWarps ? wsum[1][lane] : -1;
                 least = __reduce_min_sync(~0u, place >= 0 ? key : 0xffffffffu);
                 last = __reduce_max_sync(~0u, key == least ? place : -1);
                 if (blocks > 1) {
@@ -559,7 +562,8 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
                 const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
                 const uint32_t mask = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;        // of the digits found
                 int* mine = hist[pass & 1];
-                mine[tid] = mine[tid + kSelect] = 0;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) mine[tid + i * THREADS] = 0;
                 __syncthreads();
                 for (int w = w0; w < w1; ++w) {
                     const int t = w * 32 + lane;
@@ -567,14 +571,23 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
                     if (t < n && (key & mask) == prefix) atomicAdd(&mine[(key >> shift) & (kBins - 1)], 1);
                 }
                 sync();
-                // thread i: the bins kBins - 1 - 2 i and the one below, of all blocks
-                int2 sum = make_int2(0, 0);
+                // thread i: kPer bins of all blocks, falling from kBins - 1 - kPer i
+                int sum[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) sum[i] = 0;
                 for (int r = 0; r < blocks; ++r) {
-                    const int2 x = reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r))[kSelect - 1 - tid];
-                    sum.x += x.y;
-                    sum.y += x.x;
+                    const int2* x = reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r)) + (THREADS - 1 - tid) * (kPer / 2);
+#pragma unroll
+                    for (int i = 0; i < kPer; i += 2) {
+                        const int2 y = x[kPer / 2 - 1 - i / 2];
+                        sum[i] += y.y;
+                        sum[i + 1] += y.x;
+                    }
                 }
-                int inc = sum.x + sum.y;
+                int own = 0;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) own += sum[i];
+                int inc = own;
 #pragma unroll
                 for (int i = 1; i < 32; i *= 2) {
                     const int y = __shfl_up_sync(~0u, inc, i);
@@ -582,12 +595,19 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
                 }
                 if (lane == 31) wsum[pass & 1][warp] = inc;
                 __syncthreads();
-                const int before = inc - sum.x - sum.y + warp_sum(lane < warp ? wsum[pass & 1][lane] : 0);
-                if (before < rank && rank <= before + sum.x + sum.y) {
-                    const bool second = rank > before + sum.x;
-                    digit_s = kBins - 1 - 2 * tid - (second ? 1 : 0);
-                    rank_s = rank - before - (second ? sum.x : 0);
-                    count_s = second ? sum.y : sum.x;
+                int before = inc - own + warp_sum(lane < warp ? wsum[pass & 1][lane] : 0);
+                if (before < rank && rank <= before + own) {
+                    bool found = false;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) {
+                        if (!found && rank <= before + sum[i]) {
+                            digit_s = kBins - 1 - kPer * tid - i;
+                            rank_s = rank - before;
+                            count_s = sum[i];
+                            found = true;
+                        }
+                        before += sum[i];
+                    }
                 }
                 __syncthreads();
                 prefix |= (uint32_t)digit_s << shift;
@@ -611,7 +631,7 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
                 if (lane == 0) wsum[0][warp] = ties;
                 __syncthreads();
                 tie0 = warp_sum(lane < warp ? wsum[0][lane] : 0);
-                if (tid == kSelect - 1) block_sum[0] = tie0 + ties;
+                if (tid == THREADS - 1) block_sum[0] = tie0 + ties;
                 sync();
                 tie0 += warp_sum(lane < block ? *cluster.map_shared_rank(&block_sum[0], lane) : 0);
             }
@@ -637,7 +657,7 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
             }
             __syncthreads();
             int hole = warp_sum(lane < warp ? wsum[0][lane] : 0), mover = warp_sum(lane < warp ? wsum[1][lane] : 0);
-            if (tid == kSelect - 1) {
+            if (tid == THREADS - 1) {
                 block_sum[1] = hole + holes;
                 block_sum[2] = mover + movers;
             }
@@ -664,7 +684,7 @@ __global__ void __launch_bounds__(kSelect) evict_kernel(const __grid_constant__ 
         if (a.moves != nullptr) {
             if (block == 0 && tid == 0) a.moves[bh] = moves;
         } else {
-            move_rows<kSelect>(a, b, h, to, from, (int)((int64_t)moves * block / blocks), (int)((int64_t)moves * (block + 1) / blocks), moving);
+            move_rows<THREADS>(a, b, h, to, from, (int)((int64_t)moves * block / blocks), (int)((int64_t)moves * (block + 1) / blocks), moving);
         }
     } else if (a.moves != nullptr && block == 0 && tid == 0) {
         a.moves[bh] = 0;
@@ -795,12 +815,14 @@ extern "C" int rans_kv_evict(const RansKvCache* cache, int budget, int recent, c
     if (e != cudaSuccess) return (int)e;
     const uint64_t bit = (uint64_t)1 << (device & 63);
     if ((told.load(std::memory_order_relaxed) & bit) == 0) {
-        e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4);
+        e = cudaFuncSetAttribute(evict_kernel<kSelect>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_kernel<kSelectMany>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4);
         if (e != cudaSuccess) return (int)e;
         told.fetch_or(bit, std::memory_order_relaxed);
     }
     const int heads = cache->batch * cache->kv_heads;
-    const int rc2 = launch_after(evict_kernel, dim3(heads * p.blocks), kSelect, (size_t)p.shared_keys * 4, p.blocks, stream, a);
+    const bool many = heads > kSms;
+    const int rc2 = launch_after(many ? evict_kernel<kSelectMany> : evict_kernel<kSelect>, dim3(heads * p.blocks), many ? kSelectMany : kSelect, (size_t)p.shared_keys * 4, p.blocks, stream, a);
     if (rc2 != 0 || !p.apart) return rc2;
     return launch_after(move_kernel, dim3((4 * kSms + heads - 1) / heads, heads), kThreads, 0, 1, stream, a);
 }
