@@ -182,10 +182,11 @@ struct Attend {
         float2 ml[HP];
     };
 
-    // 4-bit tiles as they lie in the pages, copied ahead of their use; kSub of them are worked on at a time, where the
-    // registers allow two (their loop then turns half as often, and two chains of instructions run side by side).
-    static constexpr int kSub = kFp4 && NT == 1 && D <= 128 ? 2 : 1;
-    static constexpr int kStages = kSub == 2 ? 2 : 3;
+    // 4-bit tiles as they lie in the pages, copied ahead of their use; kSub of them are worked on at a time, as many as the
+    // registers allow (the loop then turns less often, and several chains of instructions run side by side: with 1 and
+    // these, 16 x 8000 tokens of 8 heads, groups of 12 heads of 128 67 -> 64 us, of 16 of 64 45 -> 42, of 8 of 64 38 -> 33).
+    static constexpr int kSub = !kFp4 || D == 256 ? 1 : NT == 1 && D == 64 ? 4 : 2;
+    static constexpr int kStages = kSub > 1 ? 2 : 3;
     struct alignas(16) Stage {
         uint8_t k[kTile * D / 2], v[kTile * D / 2], ks[kTile * kChunks], vs[kTile * kChunks];
     };
@@ -994,7 +995,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
             auto stages = sm.late[warp].stage;
             Group ahead = s;
             int ahead_nt = nt, ahead_tile = tile, ahead_x = x;
-            uint32_t valid = 0;                          // tokens of each stage's tiles, 5 bits each
+            std::conditional_t<(kStages * kSub > 6), uint64_t, uint32_t> valid = 0;      // tokens of each stage's tiles, 5 bits each
             bool fresh = true, ahead_fresh = true;
             auto copy = [&](int stage) {
 #pragma unroll
@@ -1003,7 +1004,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
                     if (ahead_fresh) u.begin(c, a.page, ahead.b, ahead.h, checked_length(c, ahead.b), ahead_tile, lane);
                     else u.advance(c, ahead.b, ahead.h, lane);
                     const int at = (stage * kSub + i) * 5;
-                    valid = (valid & ~(31u << at)) | (uint32_t)u.valid << at;
+                    valid = (valid & ~(decltype(valid)(31) << at)) | decltype(valid)(u.valid) << at;
                     A::copy_tile(stages[stage][i], c, u, lane);
                     ++ahead_x;
                     ahead_fresh = ++ahead_tile == ahead_nt;
