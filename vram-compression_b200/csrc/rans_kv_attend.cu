@@ -15,9 +15,9 @@
 //
 // Operands go from global memory straight to registers, 16 bytes a lane: the
 // order of the contraction index is free, so a lane's 8 consecutive values of a
-// key row are its operands of two consecutive k-steps, with
-// Q's registers loaded in the same order; and a lane that reads the same 8
-// columns of four value rows gets V^T's operands by one byte permute each.
+// key row are its operands of two consecutive k-steps, with Q's words loaded in the
+// same order; and a lane that reads the same 8 columns of four value rows gets V^T's
+// operands by one byte permute each.
 // Nothing is staged, so no warp waits for another while it streams.  4-bit rows are
 // staged instead (their loop is bound by instructions and has no registers to spare).
 //
@@ -31,7 +31,7 @@
 // Measured on one B200, 64 query heads on 8 of size 128: 48 uneven sequences in bf16
 // (1.58 GB) 235 us, 6.7 TB/s, the rate of a plain copy; one of 32768 tokens 30 us, of
 // which 18 us stream at 7.3 TB/s and the rest is launch, page lookups and joins; one of
-// 131071 tokens in 4 bits (143 MB) 48 us, about 420 instructions per 16 tokens; one of
+// 131071 tokens in 4 bits (143 MB) 46 us, about 415 instructions per 16 tokens; one of
 // 777 tokens on 2 heads 8.6 us.
 #include <atomic>
 #include <cmath>
@@ -384,9 +384,8 @@ struct Attend {
 
     // The queries of a head group, in the order of load_k()'s values, to the warp's place in shared memory
     // ([NT][kChunks][32 lanes]; 16 registers less than keeping them, for four wide reads a tile).  For 4-bit
-    // keys they become fp16: each head's largest value is first brought to
-    // [2^14, 2^15) by a power of two, so that nothing overflows and what is lost is
-    // below 2^-38 of it.
+    // keys they become fp16: each head's largest value is first brought to [2^14, 2^15) by a power of two, so that nothing
+    // overflows and what is lost is below 2^-38 of it.
     static __device__ __forceinline__ void begin(State& s, uint4* qs, const AttendArgs& a, int b, int head0, int heads, int lane) {
         const int g = lane >> 2, q4 = lane & 3;
 #pragma unroll
