@@ -258,6 +258,43 @@ def test_attend_past_4_gigabytes(torch, rc):
     assert (v[32768, :, 250 % 64] == 2).all() and int(cache.length) == 251
 
 
+def test_4_bit_pages_past_4_gigabytes(torch, rc):
+    """Every operator on 4-bit pages whose byte offsets need more than 32 bits."""
+    pages, kv, page, dim = 70000, 8, 64, 256                # a page is 64 KB: offsets pass 2^32 from page 65536 on
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB of free memory")
+    empty = lambda last, dtype=torch.uint8: torch.empty(pages, kv, page, *last, dtype=dtype, device="cuda")     # noqa: E731
+    table = torch.tensor([[69999, 3, 65537, 68000]], dtype=torch.int32, device="cuda")
+    zero = lambda: torch.zeros(1, dtype=torch.int32, device="cuda")     # noqa: E731
+    cache = rc.KVCache.from_tensors(empty([128]), empty([128]), table, zero(), zero(), empty([], torch.float32),
+                                    empty([], torch.int32), empty([8]), empty([8]))
+    n = 250
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(n, kv, dim, device="cuda").bfloat16() for _ in range(2))
+    cache.append(k, v, starts)
+    truth = {}
+    for name, x, got in (("k", k, cache.read(starts, n)[0]), ("v", v, cache.read(starts, n)[1])):
+        want = orc.values(*orc.quantise(x.double().cpu().numpy()))
+        assert np.array_equal(got.double().cpu().numpy(), want)
+        truth[name] = [want.transpose(1, 0, 2)]
+    q = torch.randn(1, 16, dim, device="cuda").bfloat16()
+    got = cache.attend(q, weigh=True)
+    check_attend(torch, cache, truth, q, [n], dim ** -0.5, got, cache.weight, table.cpu().numpy())
+    cache.weight[table[0].long()] = torch.rand(4, kv, page, device="cuda")
+    weight = cache.weight[table[0].long()].transpose(0, 1).reshape(kv, -1).cpu().numpy()
+    cache.evict(130, 20)
+    left = torch.tensor([0, 130], dtype=torch.int32, device="cuda")
+    k2 = cache.read(left, 130)[0].double().cpu().numpy()
+    position = cache.position[table[0].long()].transpose(0, 1).reshape(kv, -1).cpu().numpy()
+    for h in range(kv):
+        order = np.arange(n)
+        for to, of in orc.evict_moves(weight[h, :n], np.arange(n), n, 130, 20):
+            order[to] = of
+        assert np.array_equal(position[h, :130], order[:130])
+        assert np.array_equal(k2[:, h], truth["k"][0][h][order[:130]])
+    cache.check()
+
+
 # ------------------------------------------------------------------ append, read
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "mxfp4"])
 @pytest.mark.parametrize("given", ["bf16", "fp16", "fp32"])
