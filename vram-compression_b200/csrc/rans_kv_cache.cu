@@ -22,7 +22,7 @@ constexpr int kThreads = 256;
 // row (a quarter of a block of 32, so four neighbouring lanes share a scale).  A
 // thread keeps its column (head and part of the row) and goes through the block's
 // tokens, whose places are found once: what is left per 8 values is the rounding.
-// 10127 tokens of 8 heads of 128 into 4 bits and back: 30 us together, bound by
+// 10127 tokens of 8 heads of 128 into 4 bits and back: 28 us together, bound by
 // instructions; one token each of 4 sequences 2.8 us.
 
 struct RowArgs {
@@ -202,8 +202,8 @@ __device__ __forceinline__ uint32_t quantise8(const Given8<GIVEN>& y, uint32_t& 
     return to_e2m1(x);
 }
 
-template <int GIVEN>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ RowArgs a) {
+template <int GIVEN, bool FP4>
+__global__ void __launch_bounds__(kThreads, GIVEN == RANS_KV_FP32 ? 4 : 5) append_kernel(const __grid_constant__ RowArgs a) {
     __shared__ Where where[kTokens];
     __shared__ bool last;
     const RansKvCache& c = a.c;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     let_next_start();
     const int tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens), columns = c.kv_heads << a.part_shift;
     const int wide = min(columns, kThreads), t0 = a.columns(threadIdx.x), c0 = threadIdx.x - t0 * wide, step = a.columns(kThreads);
-    constexpr int kAtOnce = GIVEN == RANS_KV_FP32 ? 2 : 4;
+    constexpr int kAtOnce = 2;                     // (5 blocks an SM with 2 rows each at once: 28.3 us for the case above, 4 with 4: 29.7)
     Given8<GIVEN> in[kAtOnce][2];
     // token t0 + (first + u) * step of the block, column `col`; threads beyond step * wide have no token
     auto token_of = [&](int first, int u, int col) {
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     for (int col0 = 0; col0 < columns; col0 += wide) {
         const int col = c0 + col0, h = col >> a.part_shift, part = col & ((1 << a.part_shift) - 1);
         char *k = static_cast<char*>(c.k) + h * c.k_head, *v = static_cast<char*>(c.v) + h * c.v_head;
-        const int in_row = c.kind == RANS_KV_MXFP4 ? (part % 4 << a.part_shift) + part / 4 * 4 : part * 16;
+        const int in_row = FP4 ? (part % 4 << a.part_shift) + part / 4 * 4 : part * 16;
         for (int first = 0; first * step < tokens; first += kAtOnce) {
             if (col0 != 0 || first != 0) load(first, col);
 #pragma unroll
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
                 const Where& w = where[max(t, 0)];
                 const bool stored = t >= 0 && w.ok;
                 const int64_t place = w.place + h * c.page;
-                if (c.kind == RANS_KV_MXFP4) {
+                if constexpr (FP4) {
                     uint32_t byte[2];
                     const uint32_t k_code = quantise8(in[u][0], byte[0]), v_code = quantise8(in[u][1], byte[1]);
                     if (stored) {
@@ -301,7 +301,8 @@ __device__ __forceinline__ uint4 values8(uint32_t code, uint32_t byte) {
     return pack8(y, RANS_KV_BF16);
 }
 
-__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ RowArgs a) {
+template <bool FP4>
+__global__ void __launch_bounds__(kThreads, 6) read_kernel(const __grid_constant__ RowArgs a) {
     __shared__ Where where[kTokens];
     const RansKvCache& c = a.c;
     wait_for_previous();
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
                 x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
                 if (t >= tokens || !where[t].ok) continue;
                 const Where& w = where[t];
-                if (c.kind == RANS_KV_MXFP4) {
+                if constexpr (FP4) {
                     const int in_row = (part % 4 << a.part_shift) + part / 4 * 4;
                     const int64_t at = ((w.place + h * c.page) << (a.part_shift - 2)) + part / 4;
                     x[u][0].x = *reinterpret_cast<const uint32_t*>(k + w.k + in_row);
@@ -340,8 +341,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
                 const int t = first + u * step;
                 if (t >= tokens) continue;
                 const int64_t at = out0 + (int64_t)t * columns + col;
-                a.k_out[at] = c.kind == RANS_KV_MXFP4 ? values8(x[u][0].x, x[u][0].y) : x[u][0];
-                a.v_out[at] = c.kind == RANS_KV_MXFP4 ? values8(x[u][1].x, x[u][1].y) : x[u][1];
+                a.k_out[at] = FP4 ? values8(x[u][0].x, x[u][0].y) : x[u][0];
+                a.v_out[at] = FP4 ? values8(x[u][1].x, x[u][1].y) : x[u][1];
             }
         }
     }
@@ -766,7 +767,10 @@ extern "C" int rans_kv_append(const RansKvCache* cache, const void* k, const voi
     a.k_in = static_cast<const char*>(k);
     a.v_in = static_cast<const char*>(v);
     a.k_token = k_token; a.k_head = k_head; a.v_token = v_token; a.v_head = v_head;
-    auto kernel = given == RANS_KV_FP32 ? append_kernel<RANS_KV_FP32> : given == RANS_KV_FP16 ? append_kernel<RANS_KV_FP16> : append_kernel<RANS_KV_BF16>;
+    const bool fp4 = cache->kind == RANS_KV_MXFP4;
+    auto kernel = given == RANS_KV_FP32   ? (fp4 ? append_kernel<RANS_KV_FP32, true> : append_kernel<RANS_KV_FP32, false>)
+                  : given == RANS_KV_FP16 ? (fp4 ? append_kernel<RANS_KV_FP16, true> : append_kernel<RANS_KV_FP16, false>)
+                                          : (fp4 ? append_kernel<RANS_KV_BF16, true> : append_kernel<RANS_KV_BF16, false>);
     return launch_after(kernel, dim3(row_grid(a)), kThreads, 0, 1, stream, a);
 }
 
@@ -781,7 +785,7 @@ extern "C" int rans_kv_read(const RansKvCache* cache, void* k_out, void* v_out, 
     set_rows(a, *cache, starts, tokens);
     a.k_out = static_cast<uint4*>(k_out);
     a.v_out = static_cast<uint4*>(v_out);
-    return launch_after(read_kernel, dim3(row_grid(a)), kThreads, 0, 1, stream, a);
+    return launch_after(cache->kind == RANS_KV_MXFP4 ? read_kernel<true> : read_kernel<false>, dim3(row_grid(a)), kThreads, 0, 1, stream, a);
 }
 
 extern "C" int64_t rans_kv_evict_bytes(const RansKvCache* c, int budget) {
