@@ -138,6 +138,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 
+template <bool HALF>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    return HALF ? __half22float2(*reinterpret_cast<const __half2*>(&w)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+}
+
 __device__ __forceinline__ uint32_t pack_as(int half, float lo, float hi) {
     return half ? pack2<true>(lo, hi) : pack2<false>(lo, hi);
 }
@@ -555,7 +560,8 @@ struct Attend {
             }
     }
 
-    // P^T's operands from a tile's probabilities.
+    // P^T's operands from a tile's probabilities, rounded once.  For 4-bit values: to 2^-11, where the values themselves have
+    // two bits, outputs are mostly bf16 (2^-8), and the loop is short of instructions.
     template <bool HALF>
     static __device__ __forceinline__ void pack_probabilities(uint32_t (&pb)[NT][2], const float (&p)[NT][4]) {
 #pragma unroll
@@ -565,10 +571,25 @@ struct Attend {
         }
     }
 
+    // The same as sums of two operands, p to 2^-16 (bf16) or 2^-22 (fp16) of itself: the output's own rounding is then the
+    // only one that shows.  (One bf16 operand alone adds a quarter to the error's root mean square.)
+    template <bool HALF>
+    static __device__ __forceinline__ void split_probabilities(uint32_t (&high)[NT][2], uint32_t (&low)[NT][2], const float (&p)[NT][4]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t w = pack2<HALF>(p[t][2 * i], p[t][2 * i + 1]);
+                const float2 f = unpack2<HALF>(w);
+                high[t][i] = transpose8x8(w);
+                low[t][i] = transpose8x8(pack2<HALF>(p[t][2 * i] - f.x, p[t][2 * i + 1] - f.y));
+            }
+    }
+
     // O^T += V^T P^T.
     static __device__ __forceinline__ void accumulate(State& s, const RawV& r, const float (&p)[NT][4]) {
-        uint32_t pb[NT][2];
-        pack_probabilities<KIND == RANS_KV_FP16>(pb, p);
+        uint32_t high[NT][2], low[NT][2];
+        split_probabilities<KIND == RANS_KV_FP16>(high, low, p);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             const uint32_t* v0 = &r.v[0][j].x;
@@ -580,7 +601,10 @@ struct Attend {
                 const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
                 const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma<KIND == RANS_KV_FP16>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                for (int t = 0; t < NT; ++t) {
+                    mma<KIND == RANS_KV_FP16>(s.o[j * 4 + i][t], a0, a1, a2, a3, high[t][0], high[t][1]);
+                    mma<KIND == RANS_KV_FP16>(s.o[j * 4 + i][t], a0, a1, a2, a3, low[t][0], low[t][1]);
+                }
             }
         }
     }
@@ -699,8 +723,8 @@ struct Attend {
 
     // 4-bit: a tile whose scales are too far apart for fp16 (or that has a block of NaN): bf16 operands, any scale.
     static __device__ __forceinline__ void accumulate_wide(State& s, const CodeV& r, const float (&p)[NT][4]) {
-        uint32_t pb[NT][2];
-        pack_probabilities<false>(pb, p);
+        uint32_t high[NT][2], low[NT][2];
+        split_probabilities<false>(high, low, p);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             float f[4];
@@ -720,7 +744,10 @@ struct Attend {
                 const uint32_t a0 = pack2<false>(value(0, 2 * i), value(1, 2 * i)), a1 = pack2<false>(value(0, 2 * i + 1), value(1, 2 * i + 1));
                 const uint32_t a2 = pack2<false>(value(2, 2 * i), value(3, 2 * i)), a3 = pack2<false>(value(2, 2 * i + 1), value(3, 2 * i + 1));
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma<false>(s.o[j * 4 + i][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                for (int t = 0; t < NT; ++t) {
+                    mma<false>(s.o[j * 4 + i][t], a0, a1, a2, a3, high[t][0], high[t][1]);
+                    mma<false>(s.o[j * 4 + i][t], a0, a1, a2, a3, low[t][0], low[t][1]);
+                }
             }
         }
     }
