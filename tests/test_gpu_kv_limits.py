@@ -29,3 +29,29 @@ def test_attend_rounds_the_output_and_little_else(torch, rc, kind, dim, heads):
     size = want.abs().amax(-1, keepdim=True) if apart else 1.0             # (a row's largest blocks decide)
     rms = lambda x: float((x / size).square().mean().sqrt())                # noqa: E731
     assert rms(out - want) <= 1.02 * rms(want.to(q.dtype).double() - want)
+
+
+@pytest.mark.parametrize("lens", [[1], [300], [9000], [1, 0, 33, 700]])
+@pytest.mark.parametrize("spread", [8.0e37, 2.0 ** -70], ids=["large", "small"])
+def test_attend_over_bf16_values_near_the_ends_of_the_type(torch, rc, lens, spread):
+    """Sums of values up to the type's largest stay finite, and tiny ones keep their digits, in one part and in many."""
+    cache, truth, table = fill(torch, rc, lens, 2, 128, 16, "bf16", seed=sum(lens))
+    v = (cache.v.float() * spread).clamp(-3.38e38, 3.38e38).bfloat16()
+    cache.v.copy_(v)
+    pages = lambda b, n: torch.from_numpy(table[b, :-(-n // 16)]).long().cuda()     # noqa: E731
+    for b, n in enumerate(lens):
+        truth["v"][b] = v[pages(b, n)].transpose(0, 1).reshape(2, -1, 128)[:, :n].double().cpu().numpy() if n else truth["v"][b]
+    q = torch.randn(len(lens), 14, 128, device="cuda").bfloat16()
+    got = cache.attend(q, weigh=True)
+    check_attend(torch, cache, truth, q, lens, 128 ** -0.5, got, cache.weight, table)
+
+
+def test_attend_over_bf16_values_that_are_all_the_largest(torch, rc):
+    lens = [1, 40, 5000]
+    cache, _, _ = fill(torch, rc, lens, 1, 64, 16, "bf16", seed=1)
+    top = torch.finfo(torch.bfloat16).max
+    cache.v.fill_(top)
+    cache.v[..., ::2] = -top
+    out, _ = cache.attend(torch.randn(3, 8, 64, device="cuda").bfloat16())
+    # the exact answer is the value itself; fp32 sums are off by less than half a unit of bf16
+    assert (out[..., 1::2] == top).all() and (out[..., ::2] == -top).all()

@@ -56,9 +56,15 @@ constexpr int kGrid = kSms;
 // tokens 17.2, 16.5, 15.6 us; 32 uneven ones in 4 bits 78.7, 77.3, 76.6; one long one the same.
 constexpr int kStart = 4;
 // Probabilities are 2^(score - m) for a reference m that follows the running maximum from a distance: when a score passes
-// m + kHigh, m becomes the maximum - kRest.  Most tiles then leave O alone, the largest probability lies between 2^0 and
-// 2^15, and fp16 keeps probabilities down to 2^-36 of the largest instead of 2^-25.
-constexpr float kHigh = 15.0f, kRest = 11.0f;
+// m + kHigh, m becomes the maximum - kRest, and most tiles leave O alone.  For fp16 operands the largest probability lies
+// between 2^11 and 2^15, so that they keep probabilities down to 2^-36 of the largest instead of 2^-25.  bf16 operands need no
+// such help, and bf16 values may be as large as fp32 sums: there the largest lies between 2^-4 and 1, and sum and O are held in
+// units of 2^-30, so that no sum over the 2^30 tokens that a table may have passes the largest value among them.
+template <int KIND>
+struct Reference {
+    static constexpr bool kBf16 = KIND == RANS_KV_BF16;
+    static constexpr float kHigh = kBf16 ? 0.0f : 15.0f, kRest = kBf16 ? -4.0f : 11.0f, kUnits = kBf16 ? 1073741824.0f : 1.0f;
+};
 
 // The maximum before there is a score: finite, so that no difference of two of them is NaN.
 constexpr float kNothing = -3.0e38f;
@@ -171,6 +177,7 @@ __device__ __forceinline__ float join_factor(float m, float top) { return m == -
 template <int KIND, int D, int NT>
 struct Attend {
     static constexpr bool kFp4 = KIND == RANS_KV_MXFP4;
+    static constexpr float kHigh = Reference<KIND>::kHigh, kRest = Reference<KIND>::kRest, kUnits = Reference<KIND>::kUnits;
     static constexpr int HP = NT * 8;                         // heads of a tile, padded
     static constexpr int kChunks = D / 32;                    // 32 values of a row
     // One block of an SM's whole register file: fewer parts to join than from several blocks.  As many warps as the registers
@@ -554,7 +561,7 @@ struct Attend {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[i][t][e] = exp2_fast(sc[i][t][e] - s.m[t][e & 1]);
+                for (int e = 0; e < 4; ++e) sc[i][t][e] = exp2_fast(sc[i][t][e] - s.m[t][e & 1]) * (1.0f / kUnits);
                 s.l[t][0] += sc[i][t][0] + sc[i][t][2];
                 s.l[t][1] += sc[i][t][1] + sc[i][t][3];
             }
@@ -764,6 +771,7 @@ struct Attend {
 
     static __device__ __forceinline__ void finish_head(const AttendArgs& a, int b, int head, float m, float l) {
         const int64_t i = (int64_t)b * a.heads + head;
+        l *= kUnits;
         if (a.log_sum != nullptr) a.log_sum[i] = l > 0.0f || l != l ? m * 0.6931471805599453f + logf(l) : -INFINITY;
         if (a.weigh) a.stats[i] = make_float2(m == -INFINITY ? 0.0f : m, l > 0.0f || l != l ? 1.0f / l : 0.0f);
     }
