@@ -55,3 +55,23 @@ def test_attend_over_bf16_values_that_are_all_the_largest(torch, rc):
     out, _ = cache.attend(torch.randn(3, 8, 64, device="cuda").bfloat16())
     # the exact answer is the value itself; fp32 sums are off by less than half a unit of bf16
     assert (out[..., 1::2] == top).all() and (out[..., ::2] == -top).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("n", [1, 17, 600])
+def test_attend_with_scores_near_the_lowest_number(torch, rc, kind, n):
+    """Equal scores of -2.2e38 (finite in powers of two as well): the mean of the values."""
+    cache, truth, table = fill(torch, rc, [n], 1, 64, 16, kind, seed=n)
+    cache.k.fill_(0.0)
+    cache.k[..., 0] = 2.0 ** 10
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=cache.k.dtype)
+    q[..., 0] = -1.3046875
+    scale = 2.0 ** 117                                     # -1.3046875 * 2^127 = -2.2198e38, times log2 e -3.2026e38
+    out, log_sum = cache.attend(q, scale=scale, weigh=True)
+    want = truth["v"][0][0].mean(0)
+    size = np.abs(truth["v"][0][0]).mean(0)
+    assert (np.abs(out[0].double().cpu().numpy() - want) <= 2.0 ** -7 * size).all()
+    assert np.abs(log_sum.double().cpu().numpy() / (-1.3046875 * 2.0 ** 127) - 1).max() <= 2.0 ** -21
+    t = np.arange(n)
+    weight = cache.weight.cpu().numpy()[table[0, t // 16], 0, t % 16]
+    assert np.abs(weight * n / 4 - 1).max() <= 2.0 ** -18

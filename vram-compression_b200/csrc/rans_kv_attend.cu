@@ -66,8 +66,8 @@ struct Reference {
     static constexpr float kHigh = kBf16 ? 0.0f : 15.0f, kRest = kBf16 ? -4.0f : 11.0f, kUnits = kBf16 ? 1073741824.0f : 1.0f;
 };
 
-// The maximum before there is a score: finite, so that no difference of two of them is NaN.
-constexpr float kNothing = -3.0e38f;
+// The maximum before there is a score: finite, so that no difference of two of them is NaN, and no finite score is below it.
+constexpr float kNothing = -3.402823466e38f;
 
 struct AttendArgs {
     RansKvCache c;
