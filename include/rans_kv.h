@@ -10,8 +10,9 @@
  *
  *   blocks of 32 values x with one scale 2^e, e = clamp(floor(log2 max|x|) - 2,
  *   -63, 63), stored as the byte e + 127 (255 when the block holds a value that
- *   is not finite: the whole block then reads as NaN); each value as the e2m1
- *   code (sign, two exponent bits, one fraction bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ *   is not finite: the whole block then reads as NaN, whatever its codes; other
+ *   bytes than 64..190 and 255 do not occur); each value as the e2m1 code
+ *   (sign, two exponent bits, one fraction bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6)
  *   nearest to x / 2^e, ties to the even code, at most 6.  A row is dim/2 bytes
  *   of codes and, in arrays of their own, dim/32 scale bytes.  Value d, of block
  *   n = d / 32, lies in byte (d % 32 / 8) * dim/8 + 4 n + d % 8 / 2, in the low

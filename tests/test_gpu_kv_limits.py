@@ -75,3 +75,18 @@ def test_attend_with_scores_near_the_lowest_number(torch, rc, kind, n):
     t = np.arange(n)
     weight = cache.weight.cpu().numpy()[table[0, t // 16], 0, t % 16]
     assert np.abs(weight * n / 4 - 1).max() <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("dim,heads", [(64, 4), (128, 8), (128, 24), (256, 8)])
+def test_attend_over_key_blocks_that_are_not_finite(torch, rc, dim, heads):
+    """Scale byte 255 is NaN whatever the block's codes are: the scores, so all of the head's output, are NaN."""
+    lens = [40, 40, 40]
+    cache, _, table = fill(torch, rc, lens, 2, dim, 16, "mxfp4", seed=dim)
+    for b, code in ((0, 0x77), (1, 0xff)):                 # 6 and -6 throughout the row
+        cache.k[int(table[b, 1]), 1, 3] = code
+        cache.k_scale[int(table[b, 1]), 1, 3, 1] = 255
+    q = torch.randn(3, heads, dim, device="cuda").abs().bfloat16()
+    out, log_sum = cache.attend(q)
+    half = heads // 2
+    assert torch.isnan(out[:2, half:]).all() and torch.isnan(log_sum[:2, half:]).all()
+    assert torch.isfinite(out[:2, :half]).all() and torch.isfinite(out[2]).all() and torch.isfinite(log_sum[2]).all()

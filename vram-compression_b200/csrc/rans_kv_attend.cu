@@ -166,8 +166,13 @@ __device__ __forceinline__ uint32_t multiply2(uint32_t x, uint32_t f) {
     return *reinterpret_cast<const uint32_t*>(&z);
 }
 
-// 2^e of a scale byte e + 127 (255: infinity, whose product with the zero codes of such a block is NaN).
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// (1 + 2^-23) 2^e of byte k of a word, a scale byte e + 127, or NaN for 255: the lowest bit of the fraction, set in all, makes
+// a NaN of what would be infinity (the mask takes it along; a comparison would be two instructions more for each scale).  kOne
+// takes the factor out again.
+__device__ __forceinline__ float scale_of(uint32_t w, int k) {
+    return __uint_as_float(((k < 3 ? w << (23 - 8 * k) : w >> 1) & 0x7f800000u) | 1u);
+}
+constexpr float kOne = 1.0f - 1.1920928955078125e-7f;
 
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -432,8 +437,8 @@ struct Attend {
                         (&q[j].x)[w] = pack2<true>(f.x * down, f.y * down);
                     }
                 // a lane's scores are of heads 2 q4 and 2 q4 + 1
-                s.qs[t][0] = __shfl_sync(~0u, up, (2 * q4) * 4) * a.scale_log2;
-                s.qs[t][1] = __shfl_sync(~0u, up, (2 * q4 + 1) * 4) * a.scale_log2;
+                s.qs[t][0] = __shfl_sync(~0u, up, (2 * q4) * 4) * (a.scale_log2 * kOne);
+                s.qs[t][1] = __shfl_sync(~0u, up, (2 * q4 + 1) * 4) * (a.scale_log2 * kOne);
             }
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) qs[(t * kChunks + j) * 32 + lane] = q[j];
@@ -478,8 +483,8 @@ struct Attend {
             uint32_t w0[4], w1[4];
             e2m1_to_half(w0, r.w[0][j]);
             e2m1_to_half(w1, r.w[1][j]);
-            const float f0 = scale_of((r.s[0][j / 4] >> (8 * (j % 4))) & 255);
-            const float f1 = scale_of((r.s[1][j / 4] >> (8 * (j % 4))) & 255);
+            const float f0 = scale_of(r.s[0][j / 4], j % 4);
+            const float f1 = scale_of(r.s[1][j / 4], j % 4);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
