@@ -25,6 +25,8 @@
  * alignment, -3 when the workspace is too small.  A page number outside
  * 0..pages-1 or a length beyond the table is never followed: the token is left
  * out and a bit of *status is raised (RANS_KV_BAD_PAGE, RANS_KV_BAD_LENGTH).
+ * Rows outside `starts` and starts beyond the rows are left out and not counted;
+ * where starts fall, append adds nothing (RANS_KV_BAD_STARTS in each case).
  * Pages may be shared by sequences for attention alone; append, weigh and evict
  * want each page in one place of the table.
  * Calls on one cache share its workspace and books and have to be ordered (one

@@ -11,7 +11,7 @@ def quantise(x):
     """Rows [.., dim] -> (code value indices uint8 [.., dim] with the sign in bit 3, scale bytes [.., dim / 32]), by a
     search over the grid: the nearest value, of two equally near ones the even index."""
     x = np.asarray(x, np.float64)
-    blocks = x.reshape(*x.shape[:-1], -1, 32)
+    blocks = x.reshape(*x.shape[:-1], x.shape[-1] // 32, 32)
     finite = np.isfinite(blocks).all(-1)
     top = np.where(finite, np.abs(np.where(np.isfinite(blocks), blocks, 0)).max(-1), 0.0)
     e = np.where(top > 0, np.frexp(np.where(top > 0, top, 1.0))[1] - 3, -63).clip(-63, 63)

@@ -90,3 +90,54 @@ def test_attend_over_key_blocks_that_are_not_finite(torch, rc, dim, heads):
     half = heads // 2
     assert torch.isnan(out[:2, half:]).all() and torch.isnan(log_sum[:2, half:]).all()
     assert torch.isfinite(out[:2, :half]).all() and torch.isfinite(out[2]).all() and torch.isfinite(log_sum[2]).all()
+
+
+# ------------------------------------------------------------------ row ranges
+STARTS = {"past the rows": ([0, 2, 9], [42, 22]), "past the rows at once": ([0, 100, 200], [44, 20]),
+          "not from zero": ([1, 2, 4], [41, 22]), "from below zero": ([-3, 2, 4], [42, 22]),
+          "falling": ([0, 3, 1], [40, 20]), "falling below zero": ([0, -2, 4], [40, 20])}
+
+
+@pytest.mark.parametrize("what", list(STARTS))
+@pytest.mark.parametrize("kind", ["bf16", "mxfp4"])
+def test_append_of_bad_row_ranges_counts_what_it_stored(torch, rc, what, kind):
+    """4 rows: those inside both the ranges and the rows are stored and counted, none where the ranges fall; check() tells."""
+    starts, lens = STARTS[what]
+    cache, _, table = fill(torch, rc, [40, 20], 1, 64, 16, kind, seed=3)
+    rows = torch.randn(4, 1, 64, device="cuda").bfloat16()
+    cache.append(rows, rows, i32(torch, starts))
+    with pytest.raises(rc.CacheError, match="rows"):
+        cache.check()
+    assert cache.length.tolist() == lens and cache.seen.tolist() == lens
+    # what was counted can be read back: the rows of the clamped ranges
+    new = [n - m for n, m in zip(lens, (40, 20))]
+    got = cache.read(i32(torch, np.cumsum([0] + new)), sum(new))[0].double().cpu().numpy()
+    first = [min(max(s, 0), 4) for s in starts]
+    want = np.concatenate([rows[first[b]:first[b] + new[b]].double().cpu().numpy() for b in range(2)])
+    assert np.array_equal(got, want if kind == "bf16" else orc.values(*orc.quantise(want)))
+    cache.check()
+
+
+@pytest.mark.parametrize("starts", [[0, 2, 9], [1, 2, 4], [0, 3, 1], [-1, 2, 4]])
+def test_read_of_bad_row_ranges_is_reported(torch, rc, starts):
+    cache, truth, _ = fill(torch, rc, [40, 20], 1, 64, 16, "bf16", seed=3)
+    k, _ = cache.read(i32(torch, starts), 4)
+    assert torch.isfinite(k).all()
+    with pytest.raises(rc.CacheError, match="rows"):
+        cache.check()
+
+
+def test_append_of_falling_ranges_over_many_sequences(torch, rc):
+    """Ranges in no order over more sequences than one round of the search takes."""
+    batch = 300
+    cache, _, _ = fill(torch, rc, [5] * batch, 1, 64, 16, "bf16", seed=4)
+    rng = np.random.default_rng(0)
+    rows = torch.ones(200, 1, 64, device="cuda")
+    for _ in range(5):
+        cache.append(rows, rows, i32(torch, rng.integers(0, 201, batch + 1)))
+        with pytest.raises(rc.CacheError, match="rows"):
+            cache.check()
+        assert cache.length.tolist() == [5] * batch and cache.seen.tolist() == [5] * batch
+        assert torch.isfinite(cache.read(i32(torch, rng.integers(0, 201, batch + 1)), 200)[0]).all()
+        with pytest.raises(rc.CacheError, match="rows"):
+            cache.check()

@@ -49,8 +49,20 @@ struct Where {
     int ok;                    // 0: nowhere
 };
 
+// Sequence b's rows, as far as there are any.
 __device__ __forceinline__ int rows_of(const RowArgs& a, int b) {
-    return a.starts == nullptr ? 1 : max(a.starts[b + 1] - a.starts[b], 0);
+    return a.starts == nullptr ? 1 : max(min(a.starts[b + 1], a.tokens) - min(max(a.starts[b], 0), a.tokens), 0);
+}
+
+// Whether the rows are ranges that rise from 0 to `tokens`; a block asks, and raises what is wrong.  true: they rise, if not
+// between those two.
+__device__ __forceinline__ bool check_starts(const RowArgs& a) {
+    if (a.starts == nullptr) return true;
+    bool falls = false;
+    for (int b = threadIdx.x; b < a.c.batch; b += kThreads) falls |= a.starts[b + 1] < a.starts[b];
+    falls = __syncthreads_or(falls);
+    if (threadIdx.x == 0 && (falls || a.starts[0] != 0 || a.starts[a.c.batch] != a.tokens)) raise(a.c, RANS_KV_BAD_STARTS);
+    return !falls;
 }
 
 // The sequence b with starts[b] <= token < starts[b + 1], by the 32 lanes of a warp, and its first row; -1 if there is none.
@@ -68,6 +80,7 @@ __device__ __forceinline__ int sequence_of(const RowArgs& a, int token, int lane
         lo += of * step;
         hi = min(lo + step, hi);
     } while (hi - lo > 1);
+    first = max(first, 0);
     return __any_sync(~0u, lane == 0 ? token < edge : token >= edge) ? -1 : lo;
 }
 
@@ -83,10 +96,10 @@ __device__ __forceinline__ void find_tokens(const RowArgs& a, Where* where, bool
             if (b < 0) {
                 raise(c, RANS_KV_BAD_STARTS);
             } else {
-                const int number = token - first;
-                const int place = checked_length(c, b) + number - (last ? rows_of(a, b) : 0);
+                const int number = token - first, rows = last ? rows_of(a, b) : 0;
+                const int place = checked_length(c, b) + number - rows;
                 w.position = c.seen[b] + number;
-                if (place < 0) {
+                if (place < 0 || (last && number >= rows)) {
                     raise(c, RANS_KV_BAD_STARTS);
                 } else if (place >= (int64_t)c.table_cols * c.page) {
                     raise(c, RANS_KV_BAD_LENGTH);
@@ -279,7 +292,8 @@ __global__ void __launch_bounds__(kThreads, GIVEN == RANS_KV_FP32 ? 4 : 5) appen
         }
     }
     __syncthreads();
-    if (last)
+    // (where the ranges fall, nobody can say which rows are whose: what was stored lies behind the lengths and stays there)
+    if (last && check_starts(a))
         for (int b = threadIdx.x; b < c.batch; b += kThreads) {
             const int n = rows_of(a, b);
             c.length[b] = (int)min((int64_t)checked_length(c, b) + n, (int64_t)c.table_cols * c.page);
@@ -308,6 +322,7 @@ __global__ void __launch_bounds__(kThreads, 6) read_kernel(const __grid_constant
     wait_for_previous();
     let_next_start();
     find_tokens(a, where, true);
+    if (blockIdx.x == 0) check_starts(a);
     const int tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens), columns = c.kv_heads << a.part_shift;
     const int wide = min(columns, kThreads), t0 = a.columns(threadIdx.x), c0 = threadIdx.x - t0 * wide, step = a.columns(kThreads);
     if (t0 >= step) return;
