@@ -141,3 +141,220 @@ def test_append_of_falling_ranges_over_many_sequences(torch, rc):
         assert torch.isfinite(cache.read(i32(torch, rng.integers(0, 201, batch + 1)), 200)[0]).all()
         with pytest.raises(rc.CacheError, match="rows"):
             cache.check()
+
+
+# ------------------------------------------------------------------ pages of the cache's own
+def _rows(torch, n, kv=2, dim=64):
+    return [torch.randn(n, kv, dim, device="cuda").bfloat16() for _ in range(2)]
+
+
+def _pages_of(cache, b, n):
+    return [int(p) for p in cache.table[b, :-(-n // cache.page)]]
+
+
+def test_what_an_eviction_gives_back_is_never_shared(torch, rc):
+    """After an eviction another sequence takes the freed pages; an append without reserve by the first is left out and
+    reported, and harms nobody."""
+    cache = rc.KVCache(pages=6, page=16, kv_heads=2, dim=64, batch=2, max_tokens=96)
+    cache.reserve([64, 0])
+    cache.append(*_rows(torch, 64), i32(torch, [0, 64, 64]))
+    cache.evict(16, 4)
+    assert cache.free_pages == 5
+    cache.reserve([0, 80])                                 # all that is free
+    assert cache.free_pages == 0
+    k, v = _rows(torch, 80)
+    cache.append(k, v, i32(torch, [0, 0, 80]))
+    used = _pages_of(cache, 0, 16) + _pages_of(cache, 1, 80)
+    assert len(set(used)) == 6 and min(used) >= 0
+    cache.check()
+    cache.append(*_rows(torch, 1), i32(torch, [0, 1, 1]))  # place 16 of sequence 0: not reserved
+    got = cache.read(i32(torch, [0, 0, 80]), 80)
+    assert torch.equal(got[0], k) and torch.equal(got[1], v)
+    with pytest.raises(rc.CacheError, match="page"):
+        cache.check()
+
+
+def test_pages_reserved_for_tokens_to_come_survive_an_eviction(torch, rc):
+    cache = rc.KVCache(pages=8, page=16, kv_heads=2, dim=64, batch=2, max_tokens=128)
+    cache.reserve([100, 10])                               # 7 pages and 1
+    cache.append(*_rows(torch, 60), i32(torch, [0, 50, 60]))
+    cache.evict(32, 4)                                     # 32 left, 50 more are to come: 6 pages
+    assert cache.length.tolist() == [32, 10] and cache.free_pages == 1
+    with pytest.raises(rc.CacheError):
+        cache.reserve([0, 30])
+    k, v = _rows(torch, 50)
+    cache.append(k, v, i32(torch, [0, 50, 50]))
+    got = cache.read(i32(torch, [0, 50, 50]), 50)
+    assert torch.equal(got[0], k) and torch.equal(got[1], v)
+    assert cache.length.tolist() == [82, 10]
+    cache.check()
+    cache.evict(32, 4)                                     # of 110 tokens 10 are to come, of which sequence the host cannot tell
+    assert cache.length.tolist() == [32, 10] and cache.free_pages == 8 - 3 - 1
+    cache.check()
+
+
+def test_pages_change_hands_many_times(torch, rc):
+    """A random history of reservations, appends, evictions and releases beside what each sequence should hold."""
+    rng = np.random.default_rng(5)
+    batch, page, pages = 4, 16, 14
+    cache = rc.KVCache(pages=pages, page=page, kv_heads=1, dim=64, batch=batch, max_tokens=128, kind="fp16")
+    held = [np.zeros(0, np.int64) for _ in range(batch)]   # every token's own number, in places
+    number = 0
+    refused = 0
+    for turn in range(150):
+        what = rng.integers(0, 10)
+        if what < 6:
+            new = [int(x) for x in rng.integers(0, 30, batch)]
+            if any(len(h) + n > 128 for h, n in zip(held, new)):
+                continue
+            try:
+                cache.reserve(new)
+            except rc.CacheError:
+                refused += 1
+                assert sum(-(-(len(h) + n) // page) for h, n in zip(held, new)) > pages
+                continue
+            total = sum(new)
+            ids = np.arange(number, number + total)
+            number += total
+            rows = torch.from_numpy((ids % 2048).astype(np.float32))[:, None, None].expand(total, 1, 64).contiguous().cuda()
+            starts = np.cumsum([0] + new)
+            cache.append(rows, -rows, i32(torch, starts))
+            held = [np.concatenate([h, ids[starts[b]:starts[b + 1]]]) for b, h in enumerate(held)]
+        elif what < 9:
+            budget = int(rng.integers(1, 60))
+            cache.evict(budget, budget)                    # the newest stay, in the order of the moves
+            for b, h in enumerate(held):
+                if len(h) > budget:
+                    newest = set(np.sort(h)[-budget:])
+                    holes = [t for t in range(budget) if h[t] not in newest]
+                    movers = [t for t in range(budget, len(h)) if h[t] in newest]
+                    out = h[:budget].copy()
+                    out[holes] = h[movers]
+                    held[b] = out
+        else:
+            b = int(rng.integers(0, batch))
+            cache.release(b)
+            held[b] = held[b][:0]
+        lens = [len(h) for h in held]
+        assert cache.length.tolist() == lens
+        assert cache.free_pages == pages - sum(-(-n // page) for n in lens)
+        used = [p for b, n in enumerate(lens) for p in _pages_of(cache, b, n)]
+        assert len(set(used)) == len(used) and all(0 <= p < pages for p in used)
+        got = cache.read(i32(torch, np.cumsum([0] + lens)), sum(lens))[0][:, 0, 0].cpu().numpy()
+        assert np.array_equal(got, np.concatenate(held).astype(np.int64) % 2048)
+        cache.check()
+    assert refused > 3
+
+
+def test_a_step_at_the_budget_does_not_wait_for_the_gpu(torch, rc):
+    """Budget a multiple of the page: the page that an eviction frees is the one that the next token takes."""
+    cache = rc.KVCache(pages=20, page=16, kv_heads=2, dim=64, batch=3, max_tokens=512)
+    q = torch.randn(3, 8, 64, device="cuda").bfloat16()
+    k, v = _rows(torch, 3)
+
+    def step():
+        cache.reserve([1] * 3)
+        cache.append(k, v)
+        cache.attend(q, weigh=True)
+        cache.evict(48, 8)
+
+    for _ in range(52):
+        step()
+    torch.cuda.synchronize()
+    before = cache.table.clone()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(40):
+            step()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(cache.table, before) and cache.length.tolist() == [48] * 3 and cache.seen.tolist() == [92] * 3
+    cache.check()
+
+
+def test_new_pages_do_not_wait_for_the_gpu(torch, rc):
+    cache = rc.KVCache(pages=60, page=16, kv_heads=2, dim=64, batch=3, max_tokens=320)
+    cache.reserve([1, 0, 0])
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(12):
+            cache.reserve([17, 3, 20])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    used = [p for b, n in enumerate(cache.most) for p in _pages_of(cache, b, n)]
+    assert cache.most == [205, 36, 240] and len(set(used)) == len(used) == 13 + 3 + 15 and min(used) >= 0
+
+
+def test_a_captured_step_of_a_cache_with_pages_of_its_own(torch, rc):
+    """Append, attention and eviction of two sequences, some turns as they are and then replayed from a graph, while a third
+    one holds all pages that are free; the oracle goes along."""
+    budget, recent, steps = 48, 8, 40
+    cache = rc.KVCache(pages=11, page=16, kv_heads=2, dim=64, batch=3, max_tokens=176, kind="fp16")
+    now = [torch.zeros(n, h, 64, device="cuda", dtype=torch.float16) for n, h in ((2, 2), (2, 2), (3, 4))]
+    starts = i32(torch, [0, 1, 2, 2])
+    cache.reserve([60, 60, 0])                             # 4 pages each
+
+    def step():
+        cache.append(now[0], now[1], starts)
+        out = cache.attend(now[2], weigh=True)[0]
+        cache.evict(budget, recent)
+        return out
+
+    # what each sequence and kv head should hold, in places
+    hold = [[dict(k=np.zeros((0, 64)), v=np.zeros((0, 64)), w=np.zeros(0), p=np.zeros(0, int)) for _ in range(2)] for _ in range(2)]
+
+    def follow(seen, out):
+        k, v, q = (x.double().cpu().numpy() for x in now)
+        for b in range(2):
+            for h in range(2):
+                s = hold[b][h]
+                s["k"], s["v"] = np.vstack([s["k"], k[b, h]]), np.vstack([s["v"], v[b, h]])
+                s["w"], s["p"] = np.append(s["w"], 0.0), np.append(s["p"], seen)
+                want, _, share, size = orc.attend(q[b, 2 * h:2 * h + 2], s["k"][None], s["v"][None], 0.125)
+                got = out[b, 2 * h:2 * h + 2].double().cpu().numpy()
+                assert (np.abs(got - want) <= 2.0 ** -10 * size + 2.0 ** -24).all()
+                s["w"] = s["w"] + share[0]
+                n = len(s["p"])
+                if n > budget:
+                    # the kept ones by the cache's own weights: fp32 sums may part near ties the other way
+                    pages = torch.tensor(_pages_of(cache, b, budget)).cuda()
+                    place = cache.position[pages][:, h].reshape(-1)[:budget].cpu().numpy()
+                    assert set(range(seen + 1 - recent, seen + 1)) <= set(place.tolist())
+                    gone = sorted(set(s["p"].tolist()) - set(place.tolist()))
+                    assert len(gone) == n - budget
+                    for g in gone:
+                        i = int(np.nonzero(s["p"] == g)[0][0])
+                        old = s["p"] < seen + 1 - recent
+                        assert old[i] and s["w"][i] <= s["w"][old].min() * (1 + 1e-5)
+                        for name in s:                     # the last place moves into the freed one
+                            if i < budget:
+                                s[name][i] = s[name][-1]
+                            s[name] = s[name][:-1]
+                    assert np.array_equal(place, s["p"])
+
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    graph, out = None, None
+    for i in range(50 + steps):
+        for x in now:
+            x.normal_(generator=gen)
+        if i < 50:
+            out = step()
+        else:
+            if graph is None:
+                cache.reserve([0, 0, 48])
+                third = [r.half() for r in _rows(torch, 48)]
+                cache.append(*third, i32(torch, [0, 0, 0, 48]))
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                before = cache.length.tolist(), cache.free_pages, cache.most
+                with torch.cuda.graph(graph):
+                    out = step()
+                assert (cache.length.tolist(), cache.free_pages, cache.most) == before      # nothing ran, nothing is given back
+            graph.replay()
+        torch.cuda.synchronize()
+        follow(i, out)
+    assert cache.length.tolist() == [budget, budget, 48] and cache.seen.tolist() == [50 + steps, 50 + steps, 48]
+    got = cache.read(i32(torch, [0, 0, 0, 48]), 48)
+    assert torch.equal(got[0], third[0]) and torch.equal(got[1], third[1])
+    cache.check()

@@ -19,10 +19,13 @@ or microscaled 4-bit rows (4.25 bits a value), and runs on it:
 
 Every method but reserve, release and check is one asynchronous call on the
 current stream (capturable in a CUDA graph once the workspace has its size: run it
-once before).  Calls on one cache share its books and workspace, so they have to be
-ordered: one stream, or events between streams.  Sequences may share pages for attend
-alone; append, attend(weigh=True) and evict want every page in one place.  Page numbers and lengths are
-checked inside the kernels: what would lie outside is left out and check() raises.
+once before).  What the host knows of a cache's own pages does not move while a graph
+is captured or replayed: an eviction in a graph gives no pages back, and the pages for
+the tokens that replays append are reserved before.  Calls on one cache share its books
+and workspace, so they have to be ordered: one stream, or events between streams.
+Sequences may share pages for attend alone; append, attend(weigh=True) and evict want
+every page in one place.  Page numbers, lengths and row ranges are checked inside the
+kernels: what would lie outside is left out and check() raises.
 There is no CPU fallback.
 """
 from __future__ import annotations
@@ -87,9 +90,13 @@ class KVCache:
         self._set(rows[0], rows[1], table, torch.zeros(batch, dtype=torch.int32, device=dev),
                   torch.zeros(batch, dtype=torch.int32, device=dev), torch.zeros(shape, device=dev),
                   torch.zeros(shape, dtype=torch.int32, device=dev), scale[0], scale[1], lib)
+        # Pages: `_free` ones are in no row of the table.  `_owned` ones are in their sequence's row and in no other; those behind
+        # what the sequence needs (_needed) are free too, but stay where they are until another sequence takes them, so that a
+        # sequence at its budget, which gives a page back and takes one with every few tokens, leaves the table alone.
         self._free = list(range(pages - 1, -1, -1))
         self._owned = [[] for _ in range(batch)]
-        self._most = [0] * batch            # no sequence is longer than this
+        self._most = [0] * batch            # no sequence is longer than this, with all the tokens that are reserved
+        self._to_come = [0] * batch         # of those, no more than this are still to be appended
 
     @classmethod
     def from_tensors(cls, k, v, table, length, seen, weight=None, position=None, k_scale=None, v_scale=None, lib=None):
@@ -100,7 +107,7 @@ class KVCache:
         contiguous.  weight and position are needed by attend(weigh=True) and evict only."""
         self = cls.__new__(cls)
         self._set(k, v, table, length, seen, weight, position, k_scale, v_scale, lib)
-        self._free = self._owned = self._most = None
+        self._free = self._owned = self._most = self._to_come = None
         return self
 
     def _set(self, k, v, table, length, seen, weight, position, k_scale, v_scale, lib):
@@ -149,6 +156,7 @@ class KVCache:
         self._p = ctypes.addressof(self._c)
         self._index = self.device.index
         self._current_device, self._raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+        self._capturing = torch.cuda.is_current_stream_capturing
         self._workspaces = []               # replaced ones stay: kernels in flight may use them
         self._sizes = {}                    # what a call's shapes have been found to be good for
         self._room(self.lib.rans_kv_counter_bytes(self._p))
@@ -198,39 +206,70 @@ class KVCache:
         return starts.data_ptr()
 
     # ---------------------------------------------------------------- pages
+    def _needed(self, b):
+        return -(-self._most[b] // self.page)
+
+    def _write_table(self, entries):
+        """{(row, column): page} into the device table: one asynchronous copy from pinned memory, whatever their number."""
+        torch, cols = self._torch, self.table.shape[1]
+        at = torch.tensor([[r * cols + c for r, c in entries], list(entries.values())], dtype=torch.int64, pin_memory=True)
+        at = at.to(self.device, non_blocking=True)
+        self.table.view(-1).scatter_(0, at[0], at[1].int())
+
     def reserve(self, tokens):
-        """Hand out the pages for tokens[b] more tokens of each sequence (host; copies the table when it changed)."""
+        """Hand out the pages for tokens[b] more tokens of each sequence.  They stay reserved, whatever is evicted meanwhile,
+        until as many tokens have been appended.  (Host; one asynchronous copy where the table changes.)"""
         _need(self._free is not None, "the caller hands out the pages of a cache made from tensors")
         _need(len(tokens) == self.batch and all(t >= 0 for t in tokens), "one count per sequence")
         want = [m + t for m, t in zip(self._most, tokens)]
         _need(all(w <= self.table.shape[1] * self.page for w in want), "a sequence would outgrow max_tokens")
-        need = [max(0, -(-w // self.page) - len(o)) for w, o in zip(want, self._owned)]
-        if sum(need) > len(self._free):
-            raise CacheError(f"{sum(need)} pages needed, {len(self._free)} free")
-        for b, n in enumerate(need):
-            if n:
-                new = [self._free.pop() for _ in range(n)]
-                at = len(self._owned[b])
-                self._owned[b] += new
-                self.table[b, at:at + n] = self._torch.tensor(new, dtype=self._torch.int32).to(self.device)
+        need = [-(-w // self.page) for w in want]
+        more = sum(n - self._needed(b) for b, n in enumerate(need))
+        if more > self.free_pages:
+            raise CacheError(f"{more} pages needed, {self.free_pages} free")
         self._most = want
+        self._to_come = [t + n for t, n in zip(self._to_come, tokens)]
+        entries = {}
+        for b, n in enumerate(need):
+            own = self._owned[b]
+            while len(own) < n:
+                entries[b, len(own)] = page = self._free.pop() if self._free else self._take_back(entries)
+                own.append(page)
+        if entries:
+            self._write_table(entries)
+
+    def _take_back(self, entries):
+        """A page that a sequence no longer needs, out of the table."""
+        b = next(b for b, own in enumerate(self._owned) if len(own) > self._needed(b))
+        page = self._owned[b].pop()
+        entries[b, len(self._owned[b])] = -1
+        return page
 
     def release(self, b):
         """Forget sequence b and take its pages back."""
         _need(self._free is not None, "the caller hands out the pages of a cache made from tensors")
         self._free += reversed(self._owned[b])
-        self._owned[b], self._most[b] = [], 0
+        self._owned[b], self._most[b], self._to_come[b] = [], 0, 0
         self.table[b].fill_(-1)
         self.length[b].zero_()
         self.seen[b].zero_()
 
     @property
     def free_pages(self):
-        return len(self._free)
+        return self.pages - sum(self._needed(b) for b in range(self.batch))
+
+    def _appended(self, tokens, by_sequence):
+        """Of the reserved tokens `tokens` have come: one of each sequence, or the host does not know whose."""
+        if by_sequence:
+            self._to_come = [max(t - 1, 0) for t in self._to_come]
+        else:
+            left = max(sum(self._to_come) - tokens, 0)
+            self._to_come = [min(t, left) for t in self._to_come]
 
     @property
     def most(self):
-        """What the host knows of the lengths: no sequence is longer than this (pages reserved, less what evict gave back)."""
+        """What the host knows of the lengths: no sequence is longer than this, even with all the tokens that are reserved and
+        still to come."""
         return list(self._most)
 
     def nbytes(self):
@@ -258,6 +297,8 @@ class KVCache:
         rc = self.lib.rans_kv_append(self._p, k.data_ptr(), v.data_ptr(), given, kt, kh, vt, vh, self._starts(starts, n), n,
                                      self._stream())
         rb._check(rc, "rans_kv_append")
+        if self._free is not None and not self._capturing():
+            self._appended(n, starts is None)
 
     def read(self, starts=None, tokens=None):
         """The last starts[b+1]-starts[b] tokens of each sequence (without starts: the last one) as dense rows k, v
@@ -324,7 +365,8 @@ class KVCache:
     def evict(self, budget, recent=0):
         """Bring sequences with more than `budget` tokens back to it, per kv head: the `recent` newest tokens and the
         heaviest others stay (ties: the lower place).  Kept tokens from above the budget fill the freed places below, so
-        pages past the budget come back (to this cache's free list, or to the caller who hands them out)."""
+        pages past the budget are free again (to this cache's other sequences, or to the caller who hands them out), but for
+        those that are reserved for tokens to come."""
         _need(self.weight is not None and self.position is not None, "this cache has no weight and position tensors")
         budget, recent = int(budget), int(recent)
         _need(budget >= 1 and 0 <= recent <= budget, "budget must be positive and recent between 0 and budget")
@@ -333,13 +375,8 @@ class KVCache:
             size = self._sizes[budget] = self.lib.rans_kv_evict_bytes(self._p, budget)
             self._room(size)
         rb._check(self.lib.rans_kv_evict(self._p, budget, recent, self._stream()), "rans_kv_evict")
-        if self._free is not None:
-            keep = -(-budget // self.page)
-            for b, m in enumerate(self._most):
-                if m > budget:
-                    self._most[b] = budget
-                    self._free += reversed(self._owned[b][keep:])
-                    del self._owned[b][keep:]
+        if self._free is not None and not self._capturing():
+            self._most = [min(m, budget + t) for m, t in zip(self._most, self._to_come)]
 
     def check(self):
         """Synchronise and raise CacheError if a kernel so far met a bad page, length or row range (reading clears it)."""
