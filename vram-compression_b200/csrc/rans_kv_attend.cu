@@ -89,9 +89,11 @@ struct AttendArgs {
     int score_tiles;
 };
 
+// (Not the path for data that is constant while the kernel lives: the kernel before may still write rows when this one starts.
+// volatile: stays behind wait_for_previous().)
 __device__ __forceinline__ uint4 load16(const void* p) {
     uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
 }
@@ -262,14 +264,14 @@ struct Attend {
         __device__ __forceinline__ void fetch_next(const RansKvCache& c, int b) {
             ++ahead;
             // only a page that holds tokens is looked up (n <= table_cols * page, so `ahead` is then inside the table)
-            next = left > c.page - slot ? __ldg(c.table + (int64_t)b * c.table_cols + ahead) : -1;
+            next = left > c.page - slot ? c.table[(int64_t)b * c.table_cols + ahead] : -1;
         }
         __device__ __forceinline__ void begin(const RansKvCache& c, const Divider& page, int b, int h, int n, int tile, int lane) {
             const int t0 = tile * kTile;
             ahead = page(t0);
             slot = t0 - ahead * c.page;
             left = n - t0;
-            at_page(c, h, __ldg(c.table + (int64_t)b * c.table_cols + ahead), lane);
+            at_page(c, h, c.table[(int64_t)b * c.table_cols + ahead], lane);
             fetch_next(c, b);
         }
         __device__ __forceinline__ void advance(const RansKvCache& c, int b, int h, int lane) {
@@ -1218,8 +1220,8 @@ __global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_const
     __shared__ int warp_sum[2][kWeighThreads / 32];
     const RansKvCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // The lengths do not change during the attention before this kernel, which began when they were complete: they may be
-    // read before it ends.
+    wait_for_previous();
+    let_next_start();
     {
         const int per = (c.batch + kWeighThreads - 1) / kWeighThreads, b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
         int sum[2] = {0, 0};
@@ -1257,8 +1259,6 @@ __global__ void __launch_bounds__(kWeighThreads) weigh_kernel(const __grid_const
         if (b1 == c.batch && b0 < b1) spans[c.batch] = at[1];
         __syncthreads();
     }
-    wait_for_previous();
-    let_next_start();
     const int total = spans[c.batch] * c.kv_heads;
     for (int i = blockIdx.x * (kWeighThreads / 32) + warp; i < total; i += gridDim.x * (kWeighThreads / 32)) {
         int b = 0, hi = c.batch;

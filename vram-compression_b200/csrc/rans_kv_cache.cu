@@ -125,10 +125,11 @@ struct Given8 {
     uint4 w[GIVEN == RANS_KV_FP32 ? 2 : 1];
 };
 
+// (Plain loads: the kernel before may still write rows when this one starts, so they are not constant while it lives.)
 template <int GIVEN>
 __device__ __forceinline__ void load8(Given8<GIVEN>& x, const char* p) {
-    x.w[0] = __ldg(reinterpret_cast<const uint4*>(p));
-    if constexpr (GIVEN == RANS_KV_FP32) x.w[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    x.w[0] = *reinterpret_cast<const uint4*>(p);
+    if constexpr (GIVEN == RANS_KV_FP32) x.w[1] = *(reinterpret_cast<const uint4*>(p) + 1);
 }
 
 template <int GIVEN>
