@@ -358,3 +358,16 @@ def test_a_captured_step_of_a_cache_with_pages_of_its_own(torch, rc):
     got = cache.read(i32(torch, [0, 0, 0, 48]), 48)
     assert torch.equal(got[0], third[0]) and torch.equal(got[1], third[1])
     cache.check()
+
+
+# ------------------------------------------------------------------ eviction's workspace
+def test_evicting_to_more_than_the_table_holds(torch, rc):
+    """Nothing can be over such a budget: no lists of that size are kept."""
+    cache, _, _ = fill(torch, rc, [100, 64], 2, 64, 16, "bf16")
+    cache.weight.uniform_()
+    before = cache.k.clone(), torch.cuda.memory_allocated()
+    for budget in (10 ** 6, 2 ** 31 - 1, 112):
+        cache.evict(budget, 5)
+    assert torch.equal(torch.nan_to_num(cache.k), torch.nan_to_num(before[0])) and cache.length.tolist() == [100, 64]
+    assert torch.cuda.memory_allocated() - before[1] < 1 << 20
+    cache.check()

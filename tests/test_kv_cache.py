@@ -136,3 +136,17 @@ def test_struct_mirror_has_the_headers_layout():
     import rans_cache as rc
     assert ctypes.sizeof(rc.RansKvCache) == 12 * 8 + 6 * 8 + 8 * 4
     assert rc.RansKvCache.k_page.offset == 96 and rc.RansKvCache.pages.offset == 144 and rc.RansKvCache.kind.offset == 168
+
+
+def test_eviction_to_more_than_the_table_holds_needs_no_lists(lib):
+    """A (sequence, kv head) has at most as many moves as the budget and the places above it."""
+    c = _cache(table_cols=4)                               # 64 places
+    p = ctypes.addressof(c)
+    none = lib.rans_kv_evict_bytes(p, 64)
+    assert all(lib.rans_kv_evict_bytes(p, budget) == none for budget in (65, 10 ** 6, 2 ** 31 - 1))
+    assert none < lib.rans_kv_evict_bytes(p, 63) <= lib.rans_kv_evict_bytes(p, 32)
+    wide = _cache(table_cols=1 << 14, batch=128, kv_heads=8)
+    p = ctypes.addressof(wide)
+    room = 16 << 14
+    keys = (1 << 14) * 16 * 128 * 8 * 4                    # more than shared memory takes
+    assert lib.rans_kv_evict_bytes(p, room - 10) < lib.rans_kv_counter_bytes(p) + keys + 2 * 128 * 8 * 10 * 4 + (1 << 16)

@@ -386,8 +386,9 @@ struct EvictArgs {
     Divider page;
     int budget, recent;
     int* counter;                // [batch], zero between calls
-    int* to;                     // [batch * kv_heads][budget]: place of each move's destination
+    int* to;                     // [batch * kv_heads][lists]: place of each move's destination
     int* from;                   // and source
+    int lists;                   // the moves that the table has room for
     uint32_t* keys;              // [batch * kv_heads][table_cols * page], or NULL: in shared memory
     int* moves;                  // [batch * kv_heads]: how many, for move_kernel, or NULL: moved here
     int row_shift;               // log2 of the 16-byte pieces of a row
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ 
         auto sync = [&]() {
             if (blocks == 1) __syncthreads(); else cluster.sync();
         };
-        int *to = a.to + (int64_t)bh * k, *from = a.from + (int64_t)bh * k;
+        int *to = a.to + (int64_t)bh * a.lists, *from = a.from + (int64_t)bh * a.lists;
         int moves = 0;
         if (n - k <= kFew) {
             // A few too many, as in a loop that evicts as it appends: the lightest (of equals the last) goes, n - k times.
@@ -723,11 +724,12 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
     let_next_start();
     const int bh = blockIdx.y, moves = a.moves[bh];
     const int m0 = (int)((int64_t)moves * blockIdx.x / gridDim.x), m1 = (int)((int64_t)moves * (blockIdx.x + 1) / gridDim.x);
-    move_rows<kThreads>(a, bh / a.c.kv_heads, bh % a.c.kv_heads, a.to + (int64_t)bh * a.budget, a.from + (int64_t)bh * a.budget, m0, m1, moving);
+    move_rows<kThreads>(a, bh / a.c.kv_heads, bh % a.c.kv_heads, a.to + (int64_t)bh * a.lists, a.from + (int64_t)bh * a.lists, m0, m1, moving);
 }
 
 struct EvictPlan {
     int64_t to, from, moves, keys, bytes;
+    int lists;                       // most moves of a (sequence, kv head)
     bool apart;                      // moves in a kernel of their own
     int blocks, shared_keys;         // of a (sequence, kv head); keys a block holds in shared memory (0: in the workspace)
 };
@@ -741,13 +743,14 @@ bool plan_evict(const RansKvCache& c, int budget, EvictPlan& p) {
     while (p.blocks < kMaxCluster && heads * p.blocks * 2 <= kSms && room > (int64_t)p.blocks * kPlaces) p.blocks *= 2;
     const int64_t most = ((room + 31) / 32 / p.blocks + 1) * 32;
     p.shared_keys = most <= kMaxSharedKeys ? (int)most : 0;
+    p.lists = room > budget ? (int)(budget < room - budget ? budget : room - budget) : 0;
     p.to = counter_bytes(c);
-    p.from = p.to + up(heads * budget * 4);
-    p.moves = p.from + up(heads * budget * 4);
+    p.from = p.to + up(heads * p.lists * 4);
+    p.moves = p.from + up(heads * p.lists * 4);
     p.keys = p.moves + up(heads * 4);
     // Few heads leave SMs without a block of the selection: from 32 MB on, the moves get a grid of their own.
-    const int64_t row = c.kind == RANS_KV_MXFP4 ? c.dim / 2 : c.dim * 2, most_moves = room > budget ? (budget < room - budget ? budget : room - budget) : 0;
-    p.apart = heads * p.blocks < kSms && heads * most_moves * row * 2 >= (32 << 20);
+    const int64_t row = c.kind == RANS_KV_MXFP4 ? c.dim / 2 : c.dim * 2;
+    p.apart = heads * p.blocks < kSms && heads * p.lists * row * 2 >= (32 << 20);
     p.bytes = p.keys + (p.shared_keys ? 0 : up(heads * room * 4));
     return true;
 }
@@ -823,6 +826,7 @@ extern "C" int rans_kv_evict(const RansKvCache* cache, int budget, int recent, c
     char* ws = static_cast<char*>(cache->workspace);
     a.budget = budget;
     a.recent = recent;
+    a.lists = p.lists;
     a.counter = reinterpret_cast<int*>(ws + 256);
     a.to = reinterpret_cast<int*>(ws + p.to);
     a.from = reinterpret_cast<int*>(ws + p.from);
