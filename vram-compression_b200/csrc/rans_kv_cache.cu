@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, GIVEN == RANS_KV_FP32 ? 4 : 5) appen
     let_next_start();
     const int tokens = min(kTokens, a.tokens - (int)blockIdx.x * kTokens), columns = c.kv_heads << a.part_shift;
     const int wide = min(columns, kThreads), t0 = a.columns(threadIdx.x), c0 = threadIdx.x - t0 * wide, step = a.columns(kThreads);
-    constexpr int kAtOnce = 2;                     // (5 blocks an SM with 2 rows each at once: 28.3 us for the case above, 4 with 4: 29.7)
+    constexpr int kAtOnce = 2;                     // (5 blocks an SM with 2 rows each at once: 28.3 us for the case above, 4 with 4: 29.7; in bf16 17.3 and 18.2)
     Given8<GIVEN> in[kAtOnce][2];
     // token t0 + (first + u) * step of the block, column `col`; threads beyond step * wide have no token
     auto token_of = [&](int first, int u, int col) {
@@ -316,8 +316,10 @@ __device__ __forceinline__ uint4 values8(uint32_t code, uint32_t byte) {
     return pack8(y, RANS_KV_BF16);
 }
 
+// (Six blocks an SM for 4-bit rows; 16-bit ones then spill, and take five: 10127 tokens of 8 heads of 128 18.8 -> 16.3 us, 20000 of
+// 2 heads of 64 9.4 -> 9.2, the same as with four and 9.9.)
 template <bool FP4>
-__global__ void __launch_bounds__(kThreads, 6) read_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(kThreads, FP4 ? 6 : 5) read_kernel(const __grid_constant__ RowArgs a) {
     __shared__ Where where[kTokens];
     const RansKvCache& c = a.c;
     wait_for_previous();
