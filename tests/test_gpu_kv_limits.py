@@ -360,6 +360,31 @@ def test_a_captured_step_of_a_cache_with_pages_of_its_own(torch, rc):
     cache.check()
 
 
+def test_a_layer_lets_its_sequences_grow_by_the_slack_whatever_is_reserved(torch, rc):
+    """Pages reserved ahead are not tokens: evictions come when budget + slack are passed."""
+    import rans_model as rm
+
+    class Same(torch.nn.Module):
+        def __init__(self, rows):
+            super().__init__()
+            self.out_features, self.in_features = rows, 128
+
+        def forward(self, x):
+            return x[:, :self.out_features]
+
+    cache = rc.KVCache(pages=20, page=16, kv_heads=1, dim=64, batch=2, max_tokens=160)
+    layer = rm.RansAttention(Same(128), Same(64), Same(64), Same(128), cache, 2, budget=24, recent=8, slack=4)
+    cache.reserve([100, 60])
+    lens = []
+    for _ in range(45):
+        layer(torch.randn(2, 128, device="cuda").bfloat16())
+        lens.append(cache.length.tolist())
+        assert cache.held == lens[-1]
+    want = list(range(1, 29)) + [24, 25, 26, 27, 28] * 4
+    assert lens == [[n, n] for n in want[:45]]
+    cache.check()
+
+
 # ------------------------------------------------------------------ eviction's workspace
 def test_evicting_to_more_than_the_table_holds(torch, rc):
     """Nothing can be over such a budget: no lists of that size are kept."""

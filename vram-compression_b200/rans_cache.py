@@ -97,6 +97,7 @@ class KVCache:
         self._owned = [[] for _ in range(batch)]
         self._most = [0] * batch            # no sequence is longer than this, with all the tokens that are reserved
         self._to_come = [0] * batch         # of those, no more than this are still to be appended
+        self._held = [0] * batch            # no sequence holds more than this, unless graphs append too
 
     @classmethod
     def from_tensors(cls, k, v, table, length, seen, weight=None, position=None, k_scale=None, v_scale=None, lib=None):
@@ -107,7 +108,7 @@ class KVCache:
         contiguous.  weight and position are needed by attend(weigh=True) and evict only."""
         self = cls.__new__(cls)
         self._set(k, v, table, length, seen, weight, position, k_scale, v_scale, lib)
-        self._free = self._owned = self._most = self._to_come = None
+        self._free = self._owned = self._most = self._to_come = self._held = None
         return self
 
     def _set(self, k, v, table, length, seen, weight, position, k_scale, v_scale, lib):
@@ -156,7 +157,7 @@ class KVCache:
         self._p = ctypes.addressof(self._c)
         self._index = self.device.index
         self._current_device, self._raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
-        self._capturing = torch.cuda.is_current_stream_capturing
+        self._capturing, self._in_graphs = torch.cuda.is_current_stream_capturing, False
         self._workspaces = []               # replaced ones stay: kernels in flight may use them
         self._sizes = {}                    # what a call's shapes have been found to be good for
         self._room(self.lib.rans_kv_counter_bytes(self._p))
@@ -249,7 +250,7 @@ class KVCache:
         """Forget sequence b and take its pages back."""
         _need(self._free is not None, "the caller hands out the pages of a cache made from tensors")
         self._free += reversed(self._owned[b])
-        self._owned[b], self._most[b], self._to_come[b] = [], 0, 0
+        self._owned[b], self._most[b], self._to_come[b], self._held[b] = [], 0, 0, 0
         self.table[b].fill_(-1)
         self.length[b].zero_()
         self.seen[b].zero_()
@@ -260,6 +261,7 @@ class KVCache:
 
     def _appended(self, tokens, by_sequence):
         """Of the reserved tokens `tokens` have come: one of each sequence, or the host does not know whose."""
+        self._held = [min(h + (1 if by_sequence else tokens), m) for h, m in zip(self._held, self._most)]
         if by_sequence:
             self._to_come = [max(t - 1, 0) for t in self._to_come]
         else:
@@ -271,6 +273,12 @@ class KVCache:
         """What the host knows of the lengths: no sequence is longer than this, even with all the tokens that are reserved and
         still to come."""
         return list(self._most)
+
+    @property
+    def held(self):
+        """No sequence holds more tokens than this: what was appended, as far as the host can tell, less what was evicted.
+        Once an append has been captured in a graph: as `most`."""
+        return list(self._most if self._in_graphs else self._held)
 
     def nbytes(self):
         """Bytes of rows, scales and books."""
@@ -297,8 +305,11 @@ class KVCache:
         rc = self.lib.rans_kv_append(self._p, k.data_ptr(), v.data_ptr(), given, kt, kh, vt, vh, self._starts(starts, n), n,
                                      self._stream())
         rb._check(rc, "rans_kv_append")
-        if self._free is not None and not self._capturing():
-            self._appended(n, starts is None)
+        if self._free is not None:
+            if self._capturing():
+                self._in_graphs = True
+            else:
+                self._appended(n, starts is None)
 
     def read(self, starts=None, tokens=None):
         """The last starts[b+1]-starts[b] tokens of each sequence (without starts: the last one) as dense rows k, v
@@ -377,6 +388,7 @@ class KVCache:
         rb._check(self.lib.rans_kv_evict(self._p, budget, recent, self._stream()), "rans_kv_evict")
         if self._free is not None and not self._capturing():
             self._most = [min(m, budget + t) for m, t in zip(self._most, self._to_come)]
+            self._held = [min(h, budget) for h in self._held]
 
     def check(self):
         """Synchronise and raise CacheError if a kernel so far met a bad page, length or row range (reading clears it)."""

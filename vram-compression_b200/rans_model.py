@@ -363,6 +363,6 @@ class RansAttention(_torch_nn().nn.Module):
         c.append(k, v)
         out, _ = c.attend(q.to(torch.float16 if c.kind == "fp16" else torch.bfloat16), scale=self.scale,
                           weigh=self.budget is not None)
-        if self.budget is not None and max(c.most) > self.budget + self.slack:
+        if self.budget is not None and max(c.held) > self.budget + self.slack:
             c.evict(self.budget, self.recent)
         return self.o(out.view(c.batch, -1)).to(x.dtype)
