@@ -396,3 +396,43 @@ def test_evicting_to_more_than_the_table_holds(torch, rc):
     assert torch.equal(torch.nan_to_num(cache.k), torch.nan_to_num(before[0])) and cache.length.tolist() == [100, 64]
     assert torch.cuda.memory_allocated() - before[1] < 1 << 20
     cache.check()
+
+
+# ------------------------------------------------------------------ sharing
+@pytest.mark.parametrize("kind", ["bf16", "mxfp4"])
+def test_attend_over_shared_pages(torch, rc, kind):
+    """Two sequences with the same first pages, as after a fork, and one that is all of another's."""
+    cache, truth, table = fill(torch, rc, [100, 70, 48], 2, 128, 16, kind, seed=6)
+    table = table.copy()
+    table[1, :3] = table[0, :3]                            # 48 tokens in common
+    table[2, :3] = table[0, :3]
+    for name in "kv":
+        truth[name][1] = np.concatenate([truth[name][0][:, :48], truth[name][1][:, 48:]], 1)
+        truth[name][2] = truth[name][0][:, :48]
+    cache.table.copy_(torch.from_numpy(table))
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    check_attend(torch, cache, truth, q, [100, 70, 48], 0.03, cache.attend(q, scale=0.03))
+    cache.check()
+
+
+def test_two_caches_on_two_streams(torch, rc):
+    """Caches share nothing: the same passes side by side give the bits that they give alone."""
+    lens = [3000, 17, 900]
+    made = [fill(torch, rc, lens, 2, 128, 16, kind, seed=s)[0] for s, kind in ((1, "bf16"), (2, "mxfp4"))]
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    alone = []
+    for cache in made:
+        for _ in range(20):
+            out, log_sum = cache.attend(q, weigh=True)
+        alone.append((out, log_sum, cache.weight.clone()))
+        cache.weight.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    got = [None, None]
+    for _ in range(20):
+        for i, (cache, stream) in enumerate(zip(made, streams)):
+            with torch.cuda.stream(stream):
+                got[i] = cache.attend(q, weigh=True)
+    torch.cuda.synchronize()
+    for cache, one, two in zip(made, alone, got):
+        assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1]) and torch.equal(one[2], cache.weight)
