@@ -5,7 +5,7 @@
 // over tiles of 16 tokens and with the running maximum m and sum l of a softmax,
 //
 //     S^T = K Q^T            (tokens x heads)
-//     P^T = exp2(S^T c - m)  (c = scale * log2 e)
+//     P^T = exp2(S^T c - m)  (c = scale * log2 e; for 16-bit rows the sum of two operands, high and low)
 //     O^T = O^T 2^(m_old - m) + V^T P^T   (dim x heads)
 //
 // Both products take the cache as the 16-row operand of mma.m16n8k16 and the
@@ -29,10 +29,10 @@
 // which block that is).
 //
 // Measured on one B200, 64 query heads on 8 of size 128: 48 uneven sequences in bf16
-// (1.58 GB) 235 us, 6.7 TB/s, the rate of a plain copy; one of 32768 tokens 30 us, of
+// (1.58 GB) 236 us, 6.7 TB/s, the rate of a plain copy; one of 32768 tokens 30 us, of
 // which 18 us stream at 7.3 TB/s and the rest is launch, page lookups and joins; one of
-// 131071 tokens in 4 bits (143 MB) 46 us, about 415 instructions per 16 tokens; one of
-// 777 tokens on 2 heads 8.6 us.
+// 131071 tokens in 4 bits (143 MB) 48 us, about 425 instructions per 16 tokens, issued
+// in 55 % of the cycles; one of 777 tokens on 2 heads 8.7 us.
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -53,7 +53,7 @@ constexpr int kTile = 16;
 constexpr int kGrid = kSms;
 // A group's first tile waits for its page number and queries, and its end is written out: in the shares of work it
 // counts as this many tiles more (places without a tile behind the group's last one).  With 1, 2, 4: 200 sequences of 20
-// tokens 17.2, 16.5, 15.6 us; 32 uneven ones in 4 bits 78.7, 77.3, 76.6; one long one the same.
+// tokens 17.2, 16.5, 15.6 us; 32 uneven ones in 4 bits 78.7, 77.3, 76.6 (now 79); one long one the same.
 constexpr int kStart = 4;
 // Probabilities are 2^(score - m) for a reference m that follows the running maximum from a distance: when a score passes
 // m + kHigh, m becomes the maximum - kRest, and most tiles leave O alone.  For fp16 operands the largest probability lies
@@ -188,8 +188,9 @@ struct Attend {
     static constexpr int HP = NT * 8;                         // heads of a tile, padded
     static constexpr int kChunks = D / 32;                    // 32 values of a row
     // One block of an SM's whole register file: fewer parts to join than from several blocks.  As many warps as the registers
-    // for rows, O and statistics allow without spilling; 4-bit rows are not held in registers (12 against 8 warps: 16 x 8000
-    // tokens of 8 heads in 4 bits, groups of 12 heads of 128: 79 -> 68 us, of 8 heads of 256: 93 -> 83 us).
+    // for rows, O and statistics allow: nothing is spilled but 4 to 24 bytes a thread where 16 heads of 64 or 4-bit rows are
+    // worked on, 40 for 4-bit rows in groups of 9 to 16 heads of 128.  4-bit rows are not held in registers (12 against 8
+    // warps: 16 x 8000 tokens of 8 heads in 4 bits, groups of 12 heads of 128: 79 -> 68 us, of 8 heads of 256: 93 -> 83, now 85).
     static constexpr bool kLarge = (NT == 2 && D == 128) || D == 256;
     static constexpr int kWarps = kLarge ? (kFp4 ? 12 : 8) : D == 128 && !kFp4 ? 12 : 16;
     static constexpr int kRow = D + 4;                        // a head's part in shared memory
@@ -203,7 +204,7 @@ struct Attend {
 
     // 4-bit tiles as they lie in the pages, copied ahead of their use; kSub of them are worked on at a time, as many as the
     // registers allow (the loop then turns less often, and several chains of instructions run side by side: with 1 and
-    // these, 16 x 8000 tokens of 8 heads, groups of 12 heads of 128 67 -> 64 us, of 16 of 64 45 -> 42, of 8 of 64 38 -> 33).
+    // these, 16 x 8000 tokens of 8 heads, groups of 12 heads of 128 67 -> 64 us, now 65, of 16 of 64 45 -> 42, of 8 of 64 38 -> 33).
     static constexpr int kSub = !kFp4 || D == 256 ? 1 : NT == 1 && D == 64 ? 4 : 2;
     static constexpr int kStages = kSub > 1 ? 2 : 3;
     struct alignas(16) Stage {
@@ -1209,7 +1210,7 @@ attend_kernel(const __grid_constant__ AttendArgs a) {
 
 // weight[t] += sum over a kv head's query heads of exp2(score - m) / l.  A warp takes 64 tokens of a head at a time, each lane
 // two of them: scores are read 32 bytes a lane, the heads' m and 1 / l by one lane each.  Bound by reading the scores (4 bytes
-// a token and query head, mostly from L2): with the stores of attend_kernel 11 us of a step of 16 x 4097 tokens on 64 heads.
+// a token and query head, mostly from L2): with the stores of attend_kernel 13 us of a step of 16 x 4097 tokens on 64 heads.
 constexpr int kWeighThreads = 256;
 constexpr int kSpan = 64;
 constexpr int kWeighBlocks = 6;          // an SM

@@ -23,7 +23,7 @@ constexpr int kThreads = 256;
 // thread keeps its column (head and part of the row) and goes through the block's
 // tokens, whose places are found once: what is left per 8 values is the rounding.
 // 10127 tokens of 8 heads of 128 into 4 bits and back: 28 us together, bound by
-// instructions; one token each of 4 sequences 2.8 us.
+// instructions; one token each of 4 sequences 3.1 us.
 
 struct RowArgs {
     RansKvCache c;
@@ -371,8 +371,10 @@ __global__ void __launch_bounds__(kThreads, FP4 ? 6 : 5) read_kernel(const __gri
 // keys (passes of 11, 11 and 10 bits, of which the last is seldom needed; the blocks' histograms are added up through the
 // cluster's shared memory), mark what stays, pair
 // the i-th kept place at or above the budget with the i-th freed place below it, and move the rows.  Sources lie at or above
-// the budget and destinations below it, so moves never meet.  Bound by the passes' latency (32 x 2 heads of 4160 tokens: 12 us)
+// the budget and destinations below it, so moves never meet.  Bound by the passes' latency (32 x 2 heads of 4160 tokens: 13.5 us)
 // and, where much moves, by rows of 256 bytes read and written (8 heads of 65536 to 16384, 50 MB: 22 us to select, 24 to move).
+// Clusters, shared memory and the kernel of the moves are chosen by the table's room: these figures are of tables as long as the
+// sequences.  In tables 8 times as long 32 x 8 heads of 4160 tokens take 43 us instead of 24, 8 heads of 16385 10.4 instead of 9.2.
 
 // Threads of a block: many for a head's latency, fewer where there are more heads than SMs, so that four blocks share one (392 heads
 // of 147 tokens 18.2 -> 7.3 us, of 4200 51.3 -> 37.6; 160 of 4200 28.6 -> 26.3; but 128 of 4160 16.2 -> 22.5).

@@ -158,7 +158,7 @@ class KVCache:
         self._index = self.device.index
         self._current_device, self._raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
         self._capturing, self._in_graphs = torch.cuda.is_current_stream_capturing, False
-        self._workspaces = []               # replaced ones stay: kernels in flight may use them
+        self._workspaces = []               # replaced ones stay: kernels in flight and captured graphs may use them
         self._sizes = {}                    # what a call's shapes have been found to be good for
         self._room(self.lib.rans_kv_counter_bytes(self._p))
 
@@ -281,7 +281,7 @@ class KVCache:
         return list(self._most if self._in_graphs else self._held)
 
     def nbytes(self):
-        """Bytes of rows, scales and books."""
+        """Bytes of rows, scales and books (not of the workspace)."""
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.weight, self.position)
                    if t is not None)
 
